@@ -36,6 +36,7 @@ MODULES = {
             "attention_prefill.hip",
             "sampling.hip",
             "decode_step.hip",
+            "paged_batch.hip",
             "skinny_gemm.hip",
             "dense_gemm.hip",
             "gemm8.hip",
@@ -56,6 +57,7 @@ MODULES = {
             "activation.hip",
             "sampling.hip",
             "decode_step.hip",
+            "paged_batch.hip",
         ],
         "bindings": "bindings_seq.cpp",
         "fast_math": False,

@@ -8,7 +8,7 @@ torch. CPU tensors use the fp32 torch reference (tests, engine logic).
 
 from __future__ import annotations
 
-from typing import Optional, Tuple
+from typing import NamedTuple, Optional, Tuple
 
 import torch
 
@@ -137,19 +137,43 @@ def rotary_embedding(
     return torch_ref.rotary_embedding(positions, q, k, cos_sin_cache)
 
 
+def _both_scales(k_scale, v_scale):
+    if k_scale is None or v_scale is None:
+        raise RuntimeError("scaled pages: k_scale and v_scale go together")
+    return k_scale, v_scale
+
+
 def reshape_and_cache(
     k: torch.Tensor,
     v: torch.Tensor,
     k_cache: torch.Tensor,
     v_cache: torch.Tensor,
     slot_mapping: torch.Tensor,
+    k_scale: Optional[torch.Tensor] = None,
+    v_scale: Optional[torch.Tensor] = None,
 ) -> None:
+    """Rows k and v [tokens, kv_heads, D] into the pages of their slots.
+
+    With ``k_scale`` and ``v_scale`` (float8_e8m0fnu [pages, kv_heads]) the cache is
+    float8_e4m3fn under one power of two per page of 16 tokens and KV head. New rows ask
+    for the least that brings their largest finite value to 448 or below. A call that
+    writes a page's first row begins the page anew under it; otherwise the page keeps
+    the larger of its own and the new one, to which its other rows are rounded. Slots
+    below 0 or behind the cache are left out; of a slot given twice the later row stays.
+    Infinities become the largest number of the page."""
+    if k.is_cuda and (k_scale is not None or v_scale is not None):
+        _native("reshape_and_cache").write_scaled_pages(
+            k, v, k_cache, v_cache, *_both_scales(k_scale, v_scale), slot_mapping
+        )
+        return
     if k.is_cuda:
         _native("reshape_and_cache").reshape_and_cache(
             k, v, k_cache, v_cache, slot_mapping
         )
         return
-    torch_ref.reshape_and_cache(k, v, k_cache, v_cache, slot_mapping)
+    torch_ref.reshape_and_cache(
+        k, v, k_cache, v_cache, slot_mapping, k_scale=k_scale, v_scale=v_scale
+    )
 
 
 def paged_attention_decode(
@@ -161,7 +185,21 @@ def paged_attention_decode(
     scale: float,
     out: Optional[torch.Tensor] = None,
     window: int = 0,
+    k_scale: Optional[torch.Tensor] = None,
+    v_scale: Optional[torch.Tensor] = None,
 ) -> torch.Tensor:
+    """One query token per sequence against its pages. With ``k_scale`` and ``v_scale``
+    the pages are block-scaled (``reshape_and_cache``): heads of 64 or 128, groups of up
+    to 8; a page id outside the cache is read as its nearest page, a context longer than
+    its table row as one that fills it."""
+    if q.is_cuda and (k_scale is not None or v_scale is not None):
+        if out is None:
+            out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+        _native("paged_attention_decode").paged_attention_decode_scaled(
+            out, q, k_cache, v_cache, *_both_scales(k_scale, v_scale), block_tables,
+            context_lens, scale, window,
+        )
+        return out
     if q.is_cuda:
         if out is None:
             out = torch.empty_like(q)
@@ -172,7 +210,7 @@ def paged_attention_decode(
         return out
     return torch_ref.paged_attention_decode(
         q, k_cache, v_cache, block_tables, context_lens, scale,
-        window=window,
+        window=window, k_scale=k_scale, v_scale=v_scale,
     )
 
 
@@ -207,11 +245,22 @@ def context_attention_varlen(
     max_q_len: int,
     scale: float,
     window: int = 0,
+    k_scale: Optional[torch.Tensor] = None,
+    v_scale: Optional[torch.Tensor] = None,
 ) -> torch.Tensor:
     """Prefill attention against the paged cache (chunked prefill): the
     chunk's KV must already be written to the cache; queries attend causally
     to the whole per-seq context (bounded below by the sliding window when
-    window > 0)."""
+    window > 0). With ``k_scale`` and ``v_scale`` the pages are block-scaled
+    (``reshape_and_cache``): heads of 64 or 128; page ids and contexts are bounded as in
+    ``paged_attention_decode``."""
+    if q.is_cuda and (k_scale is not None or v_scale is not None):
+        out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+        _native("context_prefill").context_prefill_scaled(
+            out, q, k_cache, v_cache, *_both_scales(k_scale, v_scale), block_tables,
+            context_lens, cu_seqlens_q, int(max_q_len), scale, window,
+        )
+        return out
     if q.is_cuda:
         out = torch.empty_like(q)
         _native("context_prefill").context_prefill_varlen(
@@ -221,7 +270,7 @@ def context_attention_varlen(
         return out
     return torch_ref.context_attention_varlen(
         q, k_cache, v_cache, block_tables, cu_seqlens_q, context_lens, scale,
-        window=window,
+        window=window, k_scale=k_scale, v_scale=v_scale,
     )
 
 
@@ -258,6 +307,38 @@ def unpack_decode_rows(
     torch_ref.unpack_decode_rows(
         staged, width, ids, positions, context_lens, state_slots, slots, tables
     )
+
+
+class PagedBatch(NamedTuple):
+    """What attention over a paged cache is told of a batch."""
+
+    positions: torch.Tensor  # [num_tokens] int64
+    slot_mapping: torch.Tensor  # [num_tokens] int32, -1: no token
+    cu_seqlens: torch.Tensor  # [S + 1] int32
+    block_tables: torch.Tensor  # [S, max_blocks] int32
+    context_lens: torch.Tensor  # [S] int32, the new tokens among them
+    seq_of_token: torch.Tensor  # [num_tokens] int32, -1: no token
+
+
+def build_paged_batch(
+    pages: torch.Tensor, page_starts: torch.Tensor, computed_lens: torch.Tensor,
+    new_lens: torch.Tensor, num_tokens: int, max_blocks: int, block_size: int,
+) -> PagedBatch:
+    """Page tables, slots and positions of a batch from its requests' page lists
+    (``pages`` one after the other, request s's from ``page_starts[s]`` on) and lengths:
+    ``computed_lens`` tokens in pages already, ``new_lens`` to come. All int32.
+
+    ``num_tokens`` may pass the sum of the new lengths (a padded batch): rows behind the
+    last request have position 0 and slot and request -1. A token past its request's
+    pages has slot -1. Tables hold ``max_blocks`` pages of a row, 0 where it has none.
+    One kernel on the GPU."""
+    if pages.is_cuda:
+        return PagedBatch(*_native_sampling("build_paged_batch").paged_batch(
+            pages, page_starts, computed_lens, new_lens, num_tokens, max_blocks, block_size
+        ))
+    return PagedBatch(*torch_ref.build_paged_batch(
+        pages, page_starts, computed_lens, new_lens, num_tokens, max_blocks, block_size
+    ))
 
 
 def advance_decode(

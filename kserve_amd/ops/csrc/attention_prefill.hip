@@ -44,17 +44,18 @@ namespace {
 
 using namespace mfma_attn;
 
-// adds the parts of prefill_attention_kernel's keys: 32 lanes per (token, head),
-// 4 of 128 columns each. Parts without a tile wrote no sums; the others count even
+// adds the parts of prefill_attention_kernel's keys: D / 4 lanes per (token, head),
+// 4 columns each. Parts without a tile wrote no sums; the others count even
 // where their weights are NaN (by bits: a comparison of a NaN is the compiler's to
 // choose here), so that NaNs come out as from one part.
+template <int D>
 __global__ __launch_bounds__(256) void prefill_attention_merge_kernel(
     short* __restrict__ out, const float* __restrict__ part_out,
     const float* __restrict__ part_ml, const int n_splits, const long rows) {
-  constexpr int D = 128;
-  const long row = blockIdx.x * 8L + (threadIdx.x >> 5);
+  constexpr int LANES = D / 4;
+  const long row = blockIdx.x * (256L / LANES) + threadIdx.x / LANES;
   if (row >= rows) return;
-  const int d = (threadIdx.x & 31) * 4;
+  const int d = threadIdx.x % LANES * 4;
   auto empty = [](float l) {
     return __builtin_bit_cast(int, l) == __builtin_bit_cast(int, NO_KEYS);
   };
@@ -104,8 +105,9 @@ hipError_t launch(PrefillArgs p, int num_seqs, int max_q_len, bool causal,
 #undef GO
   HIP_CHECK_KERNEL();
   if (p.n_splits > 1) {
-    hipLaunchKernelGGL(prefill_attention_merge_kernel, dim3((unsigned)((p.rows + 7) / 8)),
-                       dim3(256), 0, stream, (short*)p.out, p.part_out, p.part_ml,
+    constexpr int ROWS = 256 / (D / 4);  // of a block
+    hipLaunchKernelGGL(prefill_attention_merge_kernel<D>,
+                       dim3((unsigned)((p.rows + ROWS - 1) / ROWS)), dim3(256), 0, stream, (short*)p.out, p.part_out, p.part_ml,
                        p.n_splits, p.rows);
     HIP_CHECK_KERNEL();
   }
@@ -147,6 +149,28 @@ extern "C" hipError_t ks_context_prefill_varlen(
   if (aligned16(k_cache, v_cache))
     return launch<128, PAGES_DMA>(p, num_seqs, max_q_len, true, stream);
   return launch<128, PAGES_REG>(p, num_seqs, max_q_len, true, stream);
+}
+
+extern "C" hipError_t ks_context_prefill_scaled(
+    void* out, const void* q, const void* k_cache, const void* v_cache,
+    const void* k_scale, const void* v_scale, const void* block_tables,
+    const void* ctx_lens, const void* cu_seqlens_q, int num_seqs, int max_q_len, int Hq,
+    int Hkv, int head_dim, int max_nb, int pages, float scale, long sq, int window, long rows,
+    int n_splits, void* part_out, void* part_ml, hipStream_t stream) {
+  if (Hkv < 1 || Hq < 1 || Hq % Hkv != 0 || pages < 1) return hipErrorInvalidValue;
+  if (n_splits < 1 || !part_out || !part_ml) n_splits = 1;
+  const PrefillArgs p{out, q, k_cache, v_cache,
+                      (const int*)cu_seqlens_q, (const int*)ctx_lens,
+                      (const int*)block_tables, Hq, Hkv, max_nb, 1, score_scale(scale), sq,
+                      head_dim, head_dim, window, Extra{}, n_splits, rows,
+                      (float*)part_out, (float*)part_ml,
+                      Scales{(const unsigned char*)k_scale, (const unsigned char*)v_scale,
+                             pages}};
+  if (head_dim == 128)
+    return launch<128, PAGES_FP8S>(p, num_seqs, max_q_len, true, stream);
+  if (head_dim == 64)
+    return launch<64, PAGES_FP8S>(p, num_seqs, max_q_len, true, stream);
+  return hipErrorInvalidValue;
 }
 
 extern "C" hipError_t ks_flash_prefill_varlen(

@@ -35,6 +35,18 @@ int ks_context_prefill_splits(int, long, int, int, int, int, int);
 hipError_t ks_reshape_and_cache_fp8(const void*, const void*, void*, void*,
                                     const void*, int, int, int, int, long,
                                     long, hipStream_t);
+hipError_t ks_write_scaled_pages(const void*, const void*, void*, void*, void*, void*,
+                                 const void*, long, long, int, long, long, long,
+                                 hipStream_t);
+hipError_t ks_paged_attention_decode_scaled(void*, const void*, const void*, const void*,
+                                            const void*, const void*, const void*,
+                                            const void*, float, int, int, int, int, int,
+                                            int, long, int, void*, void*, int,
+                                            hipStream_t);
+hipError_t ks_context_prefill_scaled(void*, const void*, const void*, const void*,
+                                     const void*, const void*, const void*, const void*,
+                                     const void*, int, int, int, int, int, int, int, float,
+                                     long, int, long, int, void*, void*, hipStream_t);
 hipError_t ks_embed_layer_norm(void*, const void*, const void*, const void*,
                                const void*, const void*, const void*,
                                const void*, const void*, float, int, int, int,
@@ -185,6 +197,48 @@ void reshape_and_cache(at::Tensor& k, at::Tensor& v, at::Tensor& k_cache,
             "reshape_and_cache");
 }
 
+// pages of the block-scaled cache and their scales, on device `dev`
+void check_scaled_pages(const at::Tensor& k_cache, const at::Tensor& v_cache,
+                        const at::Tensor& k_scale, const at::Tensor& v_scale,
+                        c10::Device dev) {
+  for (const at::Tensor* c : {&k_cache, &v_cache})
+    TORCH_CHECK(c->scalar_type() == at::kFloat8_e4m3fn && c->dim() == 4 &&
+                    c->size(2) == 16 && c->is_contiguous() && c->device() == dev &&
+                    c->sizes() == k_cache.sizes() && (uintptr_t)c->data_ptr() % 16 == 0,
+                "scaled pages: float8_e4m3fn [pages, kv_heads, 16, D], dense, 16-byte "
+                "aligned and on one device");
+  TORCH_CHECK(k_cache.size(3) == 64 || k_cache.size(3) == 128,
+              "scaled pages: heads of 64 or 128");
+  for (const at::Tensor* s : {&k_scale, &v_scale})
+    TORCH_CHECK(s->scalar_type() == at::kFloat8_e8m0fnu && s->dim() == 2 &&
+                    s->size(0) == k_cache.size(0) && s->size(1) == k_cache.size(1) &&
+                    s->is_contiguous() && s->device() == dev,
+                "scaled pages: scales float8_e8m0fnu [pages, kv_heads], dense");
+}
+
+void write_scaled_pages(at::Tensor& k, at::Tensor& v, at::Tensor& k_cache,
+                        at::Tensor& v_cache, at::Tensor& k_scale, at::Tensor& v_scale,
+                        at::Tensor& slot_mapping) {
+  CHECK_BF16_ROWS(k);
+  CHECK_BF16_ROWS(v);
+  const c10::Device dev = k.device();
+  const c10::DeviceGuard guard(dev);
+  check_scaled_pages(k_cache, v_cache, k_scale, v_scale, dev);
+  TORCH_CHECK(v.sizes() == k.sizes() && v.device() == dev && k.size(1) == k_cache.size(1) &&
+                  k.size(2) == k_cache.size(3),
+              "reshape_and_cache: k and v [tokens, kv_heads, D] of the pages");
+  TORCH_CHECK(slot_mapping.scalar_type() == at::kInt && slot_mapping.dim() == 1 &&
+                  slot_mapping.is_contiguous() && slot_mapping.device() == dev &&
+                  slot_mapping.size(0) >= k.size(0),
+              "slot_mapping: a dense int32 vector of the tokens");
+  check_hip(ks_write_scaled_pages(k.data_ptr(), v.data_ptr(), k_cache.data_ptr(),
+                                  v_cache.data_ptr(), k_scale.data_ptr(),
+                                  v_scale.data_ptr(), slot_mapping.data_ptr(), k.size(0),
+                                  k.size(1), (int)k.size(2), k_cache.size(0),
+                                  (long)k.stride(0), (long)v.stride(0), current_stream()),
+            "reshape_and_cache");
+}
+
 void paged_attention_decode(at::Tensor& out, at::Tensor& q,
                             at::Tensor& k_cache, at::Tensor& v_cache,
                             at::Tensor& block_tables, at::Tensor& context_lens,
@@ -221,6 +275,65 @@ void paged_attention_decode(at::Tensor& out, at::Tensor& q,
                 context_lens.data_ptr(), (float)scale, S, H, Hkv, D,
                 max_blocks, block_size, (long)q.stride(0), n_splits, po, pml,
                 (int)window, fp8 ? 1 : 0, current_stream()),
+            "paged_attention_decode");
+}
+
+// queries, tables and pages of block-scaled attention
+void check_scaled_attention(const at::Tensor& out, const at::Tensor& q,
+                            const at::Tensor& k_cache, const at::Tensor& v_cache,
+                            const at::Tensor& k_scale, const at::Tensor& v_scale,
+                            const at::Tensor& tables, const at::Tensor& ctx,
+                            int64_t seqs, int64_t window) {
+  CHECK_BF16_CONTIG(out);
+  CHECK_BF16_ROWS(q);
+  const c10::Device dev = q.device();
+  check_scaled_pages(k_cache, v_cache, k_scale, v_scale, dev);
+  TORCH_CHECK(out.sizes() == q.sizes() && out.device() == dev, "out: as the queries");
+  TORCH_CHECK(q.size(2) == k_cache.size(3) && q.size(1) >= 1 && k_cache.size(1) >= 1 &&
+                  q.size(1) % k_cache.size(1) == 0 && k_cache.size(0) >= 1 &&
+                  k_cache.size(0) < (1L << 31),
+              "scaled pages: queries [tokens, heads, D] of the pages' D, whole groups of "
+              "heads, a page at least");
+  TORCH_CHECK((q.size(0) < 2 || q.stride(0) % 8 == 0) && (uintptr_t)q.data_ptr() % 16 == 0,
+              "queries: 16-byte aligned rows");
+  TORCH_CHECK(tables.scalar_type() == at::kInt && tables.dim() == 2 &&
+                  tables.is_contiguous() && tables.device() == dev &&
+                  tables.size(0) >= seqs && tables.size(1) < (1L << 27),
+              "block_tables: dense int32 rows of the sequences");
+  TORCH_CHECK(ctx.scalar_type() == at::kInt && ctx.dim() == 1 && ctx.is_contiguous() &&
+                  ctx.device() == dev && ctx.size(0) >= seqs,
+              "context_lens: a dense int32 vector of the sequences");
+  TORCH_CHECK(window >= 0 && window < (1L << 31) && seqs < 65536 && q.size(0) < (1L << 31),
+              "scaled pages: sizes out of range");
+}
+
+void paged_attention_decode_scaled(at::Tensor& out, at::Tensor& q, at::Tensor& k_cache,
+                                   at::Tensor& v_cache, at::Tensor& k_scale,
+                                   at::Tensor& v_scale, at::Tensor& block_tables,
+                                   at::Tensor& context_lens, double scale,
+                                   int64_t window) {
+  check_scaled_attention(out, q, k_cache, v_cache, k_scale, v_scale, block_tables,
+                         context_lens, q.size(0), window);
+  const int S = q.size(0), H = q.size(1), D = q.size(2), Hkv = k_cache.size(1);
+  TORCH_CHECK(H / Hkv <= 8, "scaled pages: groups of up to 8 heads in decode");
+  const c10::DeviceGuard guard(q.device());
+  const int max_blocks = block_tables.size(1);
+  const int n_splits = ks_paged_decode_splits(S, Hkv, max_blocks, D, 1);
+  at::Tensor part_out, part_ml;
+  void *po = nullptr, *pml = nullptr;
+  if (n_splits > 1) {
+    auto opts = at::TensorOptions().dtype(at::kFloat).device(q.device());
+    part_out = at::empty({S, H, n_splits, D}, opts);
+    part_ml = at::empty({S, H, n_splits, 2}, opts);
+    po = part_out.data_ptr();
+    pml = part_ml.data_ptr();
+  }
+  check_hip(ks_paged_attention_decode_scaled(
+                out.data_ptr(), q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(),
+                k_scale.data_ptr(), v_scale.data_ptr(), block_tables.data_ptr(),
+                context_lens.data_ptr(), (float)scale, S, H, Hkv, D, max_blocks,
+                (int)k_cache.size(0), (long)q.stride(0), n_splits, po, pml, (int)window,
+                current_stream()),
             "paged_attention_decode");
 }
 
@@ -290,6 +403,45 @@ void context_prefill_varlen(at::Tensor& out, at::Tensor& q,
                 (float)scale, (long)q.stride(0), fp8, (int)window, rows, n_splits, po,
                 pml, current_stream()),
             "context_prefill_varlen");
+}
+
+void context_prefill_scaled(at::Tensor& out, at::Tensor& q, at::Tensor& k_cache,
+                            at::Tensor& v_cache, at::Tensor& k_scale, at::Tensor& v_scale,
+                            at::Tensor& block_tables, at::Tensor& ctx_lens,
+                            at::Tensor& cu_seqlens_q, int64_t max_q_len, double scale,
+                            int64_t window) {
+  TORCH_CHECK(cu_seqlens_q.scalar_type() == at::kInt && cu_seqlens_q.dim() == 1 &&
+                  cu_seqlens_q.is_contiguous() && cu_seqlens_q.size(0) >= 1 &&
+                  cu_seqlens_q.device() == q.device(),
+              "cu_seqlens_q: a dense int32 vector [sequences + 1]");
+  const int64_t seqs = cu_seqlens_q.size(0) - 1;
+  check_scaled_attention(out, q, k_cache, v_cache, k_scale, v_scale, block_tables, ctx_lens,
+                         seqs, window);
+  const c10::DeviceGuard guard(q.device());
+  const int Hq = q.size(1), Hkv = k_cache.size(1), D = q.size(2);
+  // (no sequence has more queries than there are)
+  const int longest = (int)std::min<int64_t>(std::max<int64_t>(max_q_len, 0), q.size(0));
+  const long rows = (long)q.size(0) * Hq;
+  const int n_splits =
+      ks_context_prefill_splits((int)seqs, rows, longest, Hq, Hkv,
+                                (int)block_tables.size(1), (int)window);
+  TORCH_CHECK(seqs * n_splits < 65536, "scaled pages: sizes out of range");
+  at::Tensor part_out, part_ml;
+  void *po = nullptr, *pml = nullptr;
+  if (n_splits > 1) {
+    auto opts = at::TensorOptions().dtype(at::kFloat).device(q.device());
+    part_out = at::empty({n_splits, rows, D}, opts);
+    part_ml = at::empty({n_splits, rows, 2}, opts);
+    po = part_out.data_ptr();
+    pml = part_ml.data_ptr();
+  }
+  check_hip(ks_context_prefill_scaled(
+                out.data_ptr(), q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(),
+                k_scale.data_ptr(), v_scale.data_ptr(), block_tables.data_ptr(),
+                ctx_lens.data_ptr(), cu_seqlens_q.data_ptr(), (int)seqs, longest, Hq, Hkv, D,
+                (int)block_tables.size(1), (int)k_cache.size(0), (float)scale,
+                (long)q.stride(0), (int)window, rows, n_splits, po, pml, current_stream()),
+            "context_attention_varlen");
 }
 
 void embed_layer_norm(at::Tensor& out, at::Tensor& word, at::Tensor& pos_table,
@@ -606,8 +758,14 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("silu_and_mul", &silu_and_mul, "SwiGLU activation");
   m.def("rotary_embedding", &rotary_embedding, "neox RoPE in-place");
   m.def("reshape_and_cache", &reshape_and_cache, "KV page scatter");
+  m.def("write_scaled_pages", &write_scaled_pages,
+        "K/V rows into E4M3 pages under each page's and head's scale");
   m.def("paged_attention_decode", &paged_attention_decode,
         "paged decode attention (GQA, split-context)");
+  m.def("paged_attention_decode_scaled", &paged_attention_decode_scaled,
+        "paged decode attention over block-scaled E4M3 pages");
+  m.def("context_prefill_scaled", &context_prefill_scaled,
+        "prefill attention over block-scaled E4M3 pages");
   m.def("flash_prefill_varlen", &flash_prefill_varlen,
         "MFMA flash attention (varlen GQA, causal or bidirectional)",
         pybind11::arg("out"), pybind11::arg("q"), pybind11::arg("k"),

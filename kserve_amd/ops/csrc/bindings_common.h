@@ -1,6 +1,6 @@
-// Helpers and the sampling and decode-step wrappers shared by every extension
-// module of this package (each links its own copy of sampling.hip and
-// decode_step.hip).
+// Helpers and the sampling, decode-step and batch-table wrappers shared by every
+// extension module of this package (each links its own copy of sampling.hip,
+// decode_step.hip and paged_batch.hip).
 #pragma once
 
 #include <torch/extension.h>
@@ -25,6 +25,9 @@ hipError_t ks_unpack_decode_rows(const void*, long, int, int, void*, void*, void
 hipError_t ks_advance_decode(const void*, const void*, const void*, void*, void*,
                              void*, void*, void*, void*, long, const void*, long,
                              int, int, int, hipStream_t);
+hipError_t ks_paged_batch(const void*, const void*, const void*, const void*, long, long,
+                          long, long, long, void*, void*, void*, void*, void*, void*,
+                          hipStream_t);
 }
 
 namespace {
@@ -193,10 +196,46 @@ void greedy_advance(at::Tensor& out, at::Tensor& logits, at::Tensor& ids,
             "greedy_advance");
 }
 
+// (positions, slot_mapping, cu_seqlens, block_tables, context_lens, seq_of_token)
+std::vector<at::Tensor> paged_batch(at::Tensor& pages, at::Tensor& page_starts,
+                                    at::Tensor& computed, at::Tensor& fresh,
+                                    int64_t num_tokens, int64_t max_blocks,
+                                    int64_t block_size) {
+  TORCH_CHECK(pages.is_cuda(), "pages: a GPU tensor expected");
+  const c10::Device dev = pages.device();
+  const c10::DeviceGuard guard(dev);
+  const int64_t seqs = fresh.dim() == 1 ? fresh.size(0) : 0;
+  CHECK_STEP(pages, at::kInt, 0);
+  CHECK_STEP(page_starts, at::kInt, seqs + 1);
+  CHECK_STEP(computed, at::kInt, seqs);
+  CHECK_STEP(fresh, at::kInt, 0);
+  TORCH_CHECK(page_starts.size(0) == seqs + 1 && computed.size(0) == seqs,
+              "build_paged_batch: page_starts [S + 1], computed_lens [S] and new_lens [S]");
+  TORCH_CHECK(num_tokens >= 0 && num_tokens < (1L << 31) - 1024 && max_blocks >= 0 &&
+                  block_size >= 1 && block_size < (1L << 31) &&
+                  (max_blocks == 0 || seqs <= ((1L << 31) - 1) / max_blocks),
+              "build_paged_batch: sizes out of range");
+  const auto i32 = at::TensorOptions().dtype(at::kInt).device(dev);
+  std::vector<at::Tensor> out{at::empty({num_tokens}, i32.dtype(at::kLong)),
+                              at::empty({num_tokens}, i32),
+                              at::empty({seqs + 1}, i32),
+                              at::empty({seqs, max_blocks}, i32),
+                              at::empty({seqs}, i32),
+                              at::empty({num_tokens}, i32)};
+  check_hip(ks_paged_batch(pages.data_ptr(), page_starts.data_ptr(), computed.data_ptr(),
+                           fresh.data_ptr(), pages.size(0), seqs, num_tokens, max_blocks,
+                           block_size, out[0].data_ptr(), out[1].data_ptr(),
+                           out[5].data_ptr(), out[2].data_ptr(), out[3].data_ptr(),
+                           out[4].data_ptr(), current_stream()),
+            "build_paged_batch");
+  return out;
+}
+
 void def_sampling(pybind11::module_& m) {
   m.def("unpack_decode_rows", &unpack_decode_rows, "staged decode inputs to buffers");
   m.def("advance_decode", &advance_decode, "the next decode step's inputs");
   m.def("greedy_advance", &greedy_advance, "argmax and the next decode step's inputs");
+  m.def("paged_batch", &paged_batch, "page tables, slots and positions of a batch");
   m.def("greedy_sample", &greedy_sample, "argmax sampling");
   m.def("gumbel_sample", &gumbel_sample, "Gumbel-max temperature sampling");
   m.def("topk_topp_sample", &topk_topp_sample,

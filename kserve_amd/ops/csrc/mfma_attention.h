@@ -28,7 +28,9 @@ enum Src {
   PAGES_DMA,  // bf16 pages of 16 tokens, 16-byte aligned: straight into LDS
   PAGES_REG,  // bf16 pages at any alignment: through registers
   PAGES_FP8,  // E4M3 pages, widened to bf16 on the way
+  PAGES_FP8S,  // the same under a power of two per page and KV head
 };
+constexpr bool byte_pages(int src) { return src == PAGES_FP8 || src == PAGES_FP8S; }
 
 // 16-byte chunk that chunk c of row r of a tile sits at. K fragments: 16
 // consecutive rows at one chunk must hit different banks; V fragments: 4
@@ -117,6 +119,27 @@ __device__ __forceinline__ float half_sum(float x) {
   return __uint_as_float(r[0]) + __uint_as_float(r[1]);
 }
 
+// 2^e as the widening conversions take it, from e's E8M0 byte (0, 2^-127, as the least
+// normal number: a page that holds nothing)
+__device__ __forceinline__ float page_scale(unsigned char e) {
+  return __uint_as_float(max((unsigned int)e, 1u) << 23);
+}
+
+// four E4M3 bytes each of two pages, times the pages' powers of two, as bf16 (exact: 4
+// bits of 8)
+__device__ __forceinline__ bf16x8_t widen_pages(uint2 x, float first, float second) {
+  uint4 o;
+  o.x = __builtin_bit_cast(unsigned int, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(x.x, first, false));
+  o.y = __builtin_bit_cast(unsigned int, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(x.x, first, true));
+  o.z = __builtin_bit_cast(unsigned int, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(x.y, second, false));
+  o.w = __builtin_bit_cast(unsigned int, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(x.y, second, true));
+  return __builtin_bit_cast(bf16x8_t, o);
+}
+
+__device__ __forceinline__ bf16x8_t widen_fp8(uint2 x, float scale) {
+  return widen_pages(x, scale, scale);
+}
+
 // eight E4M3 bytes as bf16 (exact)
 __device__ __forceinline__ short8_t widen_fp8(uint2 x) {
   short8_t o;
@@ -137,6 +160,13 @@ constexpr int KT = 64;      // keys per tile
 constexpr int NWAVES = 4;
 constexpr int QW = 32;      // queries per wave
 
+// What the block-scaled pages add: the exponents, and what page ids are held to.
+struct Scales {
+  const unsigned char* k;  // [NB, Hkv] E8M0
+  const unsigned char* v;
+  int pages;  // NB
+};
+
 struct PrefillArgs {
   void* out;          // [T, Hq, D]
   const void* q;      // [T, Hq, D] bf16 (PARTS 1) or fp32, row stride sq
@@ -156,6 +186,7 @@ struct PrefillArgs {
   long rows;        // T * Hq
   float* part_out;  // [n_splits, T, Hq, D]
   float* part_ml;   // [n_splits, T, Hq, 2]: exponent, sum of weights or NO_KEYS
+  Scales s8;        // PAGES_FP8S
 };
 constexpr float NO_KEYS = -1.f;  // of a part without a tile, which writes no sums
 
@@ -189,13 +220,19 @@ __global__ __launch_bounds__(256, 2) void prefill_attention_kernel(
   constexpr bool SPLITS = PAGED && PARTS == 1;
   const int seq = SPLITS ? blockIdx.z / p.n_splits : blockIdx.z;
   const int split = SPLITS ? blockIdx.z % p.n_splits : 0;
-  const int q_start = p.cu_q[seq];
-  const int q_len = p.cu_q[seq + 1] - q_start;
+  int q_start = p.cu_q[seq], q_end = p.cu_q[seq + 1];
+  if constexpr (SRC == PAGES_FP8S) {  // inside the rows whatever cu_q holds
+    const int tokens = (int)(p.rows / p.Hq);
+    q_start = min(max(q_start, 0), tokens);
+    q_end = min(q_end, tokens);
+  }
+  const int q_len = q_end - q_start;
   const int qpb = NWAVES * QW / p.hpb;  // queries per block
   // the last tiles have the most keys: they start first
   const int tile_base = (gridDim.y - 1 - blockIdx.y) * qpb;
   if (tile_base >= q_len) return;
-  const int len = PAGED ? p.ctx_lens[seq] : q_len;  // keys
+  int len = PAGED ? p.ctx_lens[seq] : q_len;  // keys
+  if constexpr (SRC == PAGES_FP8S) len = min(len, p.max_nb * PAGE);
   const int start_pos = len - q_len;                // position of query 0
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -269,14 +306,17 @@ __global__ __launch_bounds__(256, 2) void prefill_attention_kernel(
   const int* bt = PAGED ? p.block_tables + (long)seq * p.max_nb : nullptr;
   const int lrow = lane / CPR, lchunk = lane % CPR;
   auto group_of = [&](int t) { return min(t * KT + wave * 16, len - 1); };
-  auto page_of = [&](int t) { return PAGED ? bt[group_of(t) >> 4] : 0; };
+  auto page_of = [&](int t) {
+    const int id = PAGED ? bt[group_of(t) >> 4] : 0;
+    return SRC == PAGES_FP8S ? min(max(id, 0), p.s8.pages - 1) : id;
+  };
   // A scalar base per tile and 32-bit lane offsets (the launchers see to strides
   // below 2^26): tiles with all their keys cost no vector arithmetic, where 64-bit
   // addresses per lane and load took 500 of a tile's 1800 vector cycles. (As buffer
   // loads they would leave the compiler's waits for a wave's LDS reads one after the
   // other: 1 x 8191 tokens 564 -> 550 us, 64 texts of 123 tokens with heads of 64 13.3 ->
   // 14.1; the check of the waits ahead of the barriers reads the global form.)
-  constexpr int ES = SRC == PAGES_FP8 ? 1 : 2;
+  constexpr int ES = byte_pages(SRC) ? 1 : 2;
   const int krs = PAGED && PARTS == 1 ? D : (int)p.sk;  // bf16 queries: whole rows
   const int vrs = PAGED && PARTS == 1 ? D : (int)p.sv;
   // (three parts leave no registers for them: there they are formed per tile)
@@ -293,8 +333,9 @@ __global__ __launch_bounds__(256, 2) void prefill_attention_kernel(
                           : (long)(q_start + g0) * stride + kvh * D;
     return reinterpret_cast<const char*>(base) + at * ES;
   };
-  uint2 raw8[SRC == PAGES_FP8 ? 2 * NI : 1];
-  short8_t raw16[!DMA && SRC != PAGES_FP8 ? 2 * NI : 1];
+  uint2 raw8[byte_pages(SRC) ? 2 * NI : 1];
+  unsigned char exps[2];  // PAGES_FP8S: of the rows in raw8 (a wave's are one page's)
+  short8_t raw16[!DMA && !byte_pages(SRC) ? 2 * NI : 1];
   // DMA: fills buffer `buf`; otherwise the rows wait in registers for commit()
   auto stage_rows = [&](const char* kb, const char* vb, auto k_at, auto v_at, int buf) {
 #pragma unroll
@@ -308,7 +349,7 @@ __global__ __launch_bounds__(256, 2) void prefill_attention_kernel(
         __builtin_amdgcn_global_load_lds(reinterpret_cast<const unsigned int*>(vb + va),
                                          reinterpret_cast<unsigned int*>(&lds[buf][1][at]),
                                          16, 0, 0);
-      } else if constexpr (SRC == PAGES_FP8) {
+      } else if constexpr (byte_pages(SRC)) {
         raw8[2 * i] = *reinterpret_cast<const uint2*>(kb + ka);
         raw8[2 * i + 1] = *reinterpret_cast<const uint2*>(vb + va);
       } else {
@@ -321,6 +362,10 @@ __global__ __launch_bounds__(256, 2) void prefill_attention_kernel(
     const int g0 = PAGED ? group_of(t) & ~15 : group_of(t);
     const char* kb = base_of(p.k, krs, g0, page);
     const char* vb = base_of(p.v, vrs, g0, page);
+    if constexpr (SRC == PAGES_FP8S) {
+      exps[0] = p.s8.k[(long)page * p.Hkv + kvh];
+      exps[1] = p.s8.v[(long)page * p.Hkv + kvh];
+    }
     if (KEEP && (t + 1) * KT <= len)
       stage_rows(kb, vb, [&](int i) { return koff[i]; }, [&](int i) { return voff[i]; }, buf);
     else
@@ -345,6 +390,8 @@ __global__ __launch_bounds__(256, 2) void prefill_attention_kernel(
         for (int kv = 0; kv < 2; ++kv) {
           short8_t x;
           if constexpr (SRC == PAGES_FP8) x = widen_fp8(raw8[2 * i + kv]);
+          else if constexpr (SRC == PAGES_FP8S)
+            x = __builtin_bit_cast(short8_t, widen_fp8(raw8[2 * i + kv], page_scale(exps[kv])));
           else x = raw16[2 * i + kv];
           *reinterpret_cast<short8_t*>(&lds[buf][kv][at]) = x;
         }
@@ -637,7 +684,7 @@ __device__ __forceinline__ uint4 load16_nt(const char* from) {
 // launches with four use all of them: bf16 pages a pair for each (the LDS of the other
 // two is taken in any case).
 constexpr int WAVES = 2;
-constexpr int deep_pairs(int src) { return src == PAGES_FP8 ? 16 : 2 * WAVES; }
+constexpr int deep_pairs(int src) { return byte_pages(src) ? 16 : 2 * WAVES; }
 
 struct DecodeArgs {
   void* out;                // [S, H, D]
@@ -656,7 +703,24 @@ struct DecodeArgs {
   long sk, sv;
   const int* cu_q;  // [S+1] first token of a sequence (null: sequence s's is s)
   Extra x;
+  Scales s8;  // PAGES_FP8S
 };
+
+// keys of sequence s; of block-scaled pages as many as its table row has at most
+template <int SRC>
+__device__ __forceinline__ int context_of(const DecodeArgs& p, int s) {
+  return SRC == PAGES_FP8S ? min(p.ctx_lens[s], p.max_blocks * PAGE) : p.ctx_lens[s];
+}
+
+// 16-byte chunk that chunk c of a staged row of E4M3 pages is XORed with. Block-scaled
+// ones: the rows of both pages that one transposing load brings lie apart too, and heads
+// of 64 have four chunks.
+template <int D, int SRC>
+__device__ __forceinline__ int byte_swz(int r) {
+  if constexpr (SRC == PAGES_FP8) return (r >> 1) & 7;
+  else if constexpr (D == 128) return ((r >> 1) & 7) ^ (r >> 4 & 1) << 2;
+  else return ((r >> 2) & 3) ^ (r >> 4 & 1) << 1;
+}
 
 // query token of sequence s, -1 if it has none in this batch
 __device__ __forceinline__ int token_of(const DecodeArgs& p, int s) {
@@ -685,22 +749,23 @@ __device__ __forceinline__ float final_factor(const DecodeArgs& p, long tok, int
 // E4M3 pages: four waves per SIMD at least, or the compiler keeps the output in
 // accumulation registers and copies it out and back for every rescale.
 template <int D, int NW, int SRC, bool WIDE, int PARTS = 1>  // WIDE: groups of 6 to 8
-__global__ __launch_bounds__(NW * 64, SRC == PAGES_FP8 ? 4 : 1) void paged_attention_kernel(
+__global__ __launch_bounds__(NW * 64, byte_pages(SRC) ? 4 : 1) void paged_attention_kernel(
     const DecodeArgs p) {
   constexpr int KC = D / 32;           // contraction chunks of K Q^T
   constexpr int DB = D / 16;           // 16-column blocks of the output
   constexpr int ROWS = 2 * PAGE;       // rows of a stage (a pair of pages)
-  constexpr int ES = SRC == PAGES_FP8 ? 1 : 2;
+  constexpr bool BYTES = byte_pages(SRC);
+  constexpr int ES = BYTES ? 1 : 2;
   constexpr int STAGE = ROWS * D * ES;  // shorts: K rows, then V rows
   static_assert(SRC != PAGES_FP8 || D == 128, "E4M3 rows are 8 chunks");
   // elements per lane and load, loads per stage and tensor
-  constexpr int EPL = SRC == PAGES_FP8 ? 16 : 8;
+  constexpr int EPL = BYTES ? 16 : 8;
   constexpr int LPR = D / EPL;  // lanes per row
   constexpr int RPI = 64 / LPR;
   constexpr int NI = ROWS / RPI;
 
   const int kvh = blockIdx.x, s = blockIdx.y, split = blockIdx.z;
-  const int ctx = p.ctx_lens[s];
+  const int ctx = context_of<SRC>(p, s);
   const Range rg = page_range(ctx, p.window, p.x.chunk, p.n_splits, min(NW, WAVES));
   const int tok = token_of(p, s);
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -755,6 +820,8 @@ __global__ __launch_bounds__(NW * 64, SRC == PAGES_FP8 ? 4 : 1) void paged_atten
   // page ids of pair n (past the end: the last page again, as its rows are)
   auto pages_of = [&](int n) {
     const int a = min(rg.first + 2 * n, rg.last), b = min(a + 1, rg.last);
+    if constexpr (SRC == PAGES_FP8S)
+      return Pages{min(max(bt[a], 0), p.s8.pages - 1), min(max(bt[b], 0), p.s8.pages - 1)};
     return Pages{bt[a], bt[b]};
   };
   // where this lane's bytes of load i come from; rows past the context repeat
@@ -769,8 +836,17 @@ __global__ __launch_bounds__(NW * 64, SRC == PAGES_FP8 ? 4 : 1) void paged_atten
            (row * (int)st + chunk * EPL) * ES;
   };
   uint4 raw[2 * NI];
+  unsigned char exps[4];  // of the pair in raw: K of both pages, V of both
   auto load = [&](int n) {
     const Pages pg = pages_of(n);
+    if constexpr (SRC == PAGES_FP8S) {
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const long at = (long)(h ? pg.b : pg.a) * p.Hkv + kvh;
+        exps[h] = p.s8.k[at];
+        exps[2 + h] = p.s8.v[at];
+      }
+    }
 #pragma unroll
     for (int i = 0; i < NI; ++i) {
       raw[2 * i] = load16_nt(src(p.k_cache, p.sk, n, pg, i, lchunk));
@@ -784,7 +860,7 @@ __global__ __launch_bounds__(NW * 64, SRC == PAGES_FP8 ? 4 : 1) void paged_atten
 #pragma unroll
       for (int kv = 0; kv < 2; ++kv) {
         char* row = reinterpret_cast<char*>(lds[wave]) + (kv * ROWS + r) * D * ES;
-        const int sw = SRC == PAGES_FP8 ? (r >> 1) & 7 : kv ? v_swz<D>(r) : k_swz<D>(r);
+        const int sw = BYTES ? byte_swz<D, SRC>(r) : kv ? v_swz<D>(r) : k_swz<D>(r);
         *reinterpret_cast<uint4*>(row + (lchunk ^ sw) * 16) = raw[2 * i + kv];
       }
     }
@@ -795,30 +871,21 @@ __global__ __launch_bounds__(NW * 64, SRC == PAGES_FP8 ? 4 : 1) void paged_atten
   int kaddr[KC];
 #pragma unroll
   for (int c = 0; c < KC; ++c)
-    kaddr[c] = SRC == PAGES_FP8
-                   ? col * D + ((2 * c + (g >> 1)) ^ (col >> 1)) * 16 + (g & 1) * 8
+    kaddr[c] = BYTES
+                   ? col * D + ((2 * c + (g >> 1)) ^ byte_swz<D, SRC>(col)) * 16 + (g & 1) * 8
                    : (col * D + ((4 * c + g) ^ k_swz<D>(col)) * 8) * 2;
   // Transposing load: lane i of 16 brings key i/4, columns 4 (i%4) .. + 3 and
   // receives column i of its four keys; of E4M3 key i/2, columns 8 (i%2) .. + 7 and
   // column i of eight keys, the fragment's of both pages.
-  const int vrow = SRC == PAGES_FP8 ? (col >> 3) * PAGE + g * 4 + ((col >> 1) & 3)
+  const int vrow = BYTES ? (col >> 3) * PAGE + g * 4 + ((col >> 1) & 3)
                                     : g * 4 + (col >> 2);
   int vaddr[DB];
 #pragma unroll
   for (int b = 0; b < DB; ++b)
-    vaddr[b] = SRC == PAGES_FP8
-                   ? (ROWS + vrow) * D + (b ^ ((vrow >> 1) & 7)) * 16 + (col & 1) * 8
+    vaddr[b] = BYTES
+                   ? (ROWS + vrow) * D + (b ^ byte_swz<D, SRC>(vrow)) * 16 + (col & 1) * 8
                    : (ROWS * D + vrow * D + ((2 * b + ((col & 3) >> 1)) ^ v_swz<D>(vrow)) * 8 +
                       (col & 1) * 4) * 2;
-  auto widen = [](uint2 x) {  // eight E4M3 bytes, exactly
-    uint4 o;
-    o.x = __builtin_bit_cast(unsigned int, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(x.x, 1.0f, false));
-    o.y = __builtin_bit_cast(unsigned int, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(x.x, 1.0f, true));
-    o.z = __builtin_bit_cast(unsigned int, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(x.y, 1.0f, false));
-    o.w = __builtin_bit_cast(unsigned int, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(x.y, 1.0f, true));
-    return __builtin_bit_cast(bf16x8_t, o);
-  };
-
   float c2 = p.scale * LOG2E;
   const bool flip = c2 < 0.f;
   c2 = fabsf(c2);
@@ -828,6 +895,9 @@ __global__ __launch_bounds__(NW * 64, SRC == PAGES_FP8 ? 4 : 1) void paged_atten
 #pragma unroll
   for (int b = 0; b < DB; ++b) o[b] = f32x4_t{0.f, 0.f, 0.f, 0.f};
 
+  float pow2[4];  // of the pair that is multiplied: K of both pages, V of both
+#pragma unroll
+  for (int i = 0; i < 4; ++i) pow2[i] = 1.f;
   auto compute = [&](int n, const char* st) {
     f32x4_t sc[2];
 #pragma unroll
@@ -836,9 +906,11 @@ __global__ __launch_bounds__(NW * 64, SRC == PAGES_FP8 ? 4 : 1) void paged_atten
       f32x4_t rest = sc[h];  // the products with the query's lower parts
 #pragma unroll
       for (int c = 0; c < KC; ++c) {
-        const char* from = st + h * PAGE * D * ES + kaddr[c];
+        // (block-scaled: the second page's chunks are swizzled by half a row more)
+        const int at = SRC == PAGES_FP8S ? c ^ (h * KC / 2) : c;
+        const char* from = st + h * PAGE * D * ES + kaddr[at];
         bf16x8_t a;
-        if constexpr (SRC == PAGES_FP8) a = widen(*reinterpret_cast<const uint2*>(from));
+        if constexpr (BYTES) a = widen_fp8(*reinterpret_cast<const uint2*>(from), pow2[h]);
         else a = *reinterpret_cast<const bf16x8_t*>(from);
         if constexpr (PARTS == 3) {
           rest = mfma16x16x32(a, qf[PARTS - 1][c], rest);
@@ -875,7 +947,7 @@ __global__ __launch_bounds__(NW * 64, SRC == PAGES_FP8 ? 4 : 1) void paged_atten
     }
     const float mc = m * c2;
     bf16x8_t pf, pl;
-    if constexpr (WIDE || SRC == PAGES_FP8) {
+    if constexpr (WIDE || BYTES) {
 #pragma unroll
       for (int h = 0; h < 2; ++h)
 #pragma unroll
@@ -917,10 +989,12 @@ __global__ __launch_bounds__(NW * 64, SRC == PAGES_FP8 ? 4 : 1) void paged_atten
         bf16x8_t v;
       } a;
       const char* a0 = st + vaddr[b];
-      if constexpr (SRC == PAGES_FP8) {
+      if constexpr (BYTES) {
         typedef int i2_t __attribute__((ext_vector_type(2)));
         typedef __attribute__((address_space(3))) i2_t lds2_t;
-        a.v = widen(__builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr8_b64_v2i32((lds2_t*)a0)));
+        a.v = widen_pages(
+            __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr8_b64_v2i32((lds2_t*)a0)),
+            pow2[2], pow2[3]);
       } else {
         typedef __attribute__((address_space(3))) s16x4_t lds4_t;
         a.h[0] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4_t*)a0);
@@ -937,6 +1011,10 @@ __global__ __launch_bounds__(NW * 64, SRC == PAGES_FP8 ? 4 : 1) void paged_atten
   // the next pair's loads are under way while this one is multiplied
   for (int n = n_lo; n < n_hi; n += nw) {
     commit();
+    if constexpr (SRC == PAGES_FP8S) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) pow2[i] = page_scale(exps[i]);
+    }
     if (n + nw < n_hi) load(n + nw);
     compute(n, reinterpret_cast<const char*>(lds[wave]));
   }
@@ -997,7 +1075,7 @@ __global__ __launch_bounds__(NW * 64, SRC == PAGES_FP8 ? 4 : 1) void paged_atten
 
 // Combine split-context partials: one wave per (seq, head); a lane owns D/64
 // columns across all splits. Sequences that one split covers are done.
-template <int D, int NW, int PARTS = 1>
+template <int D, int NW, int PARTS = 1, int SRC = PAGES_REG>
 __global__ __launch_bounds__(256) void paged_attention_reduce_kernel(
     const DecodeArgs p, long total) {
   constexpr int ACC = D / 64;
@@ -1005,7 +1083,7 @@ __global__ __launch_bounds__(256) void paged_attention_reduce_kernel(
   const int lane = threadIdx.x & 63;
   if (sh >= total) return;
   const int s = sh / p.H;
-  const Range rg = page_range(p.ctx_lens[s], p.window, p.x.chunk, p.n_splits, min(NW, WAVES));
+  const Range rg = page_range(context_of<SRC>(p, s), p.window, p.x.chunk, p.n_splits, min(NW, WAVES));
   const int tok = token_of(p, s);
   if (rg.splits == 1 || tok < 0) return;
   const float* ml = p.part_ml + sh * p.n_splits * 2;
@@ -1079,14 +1157,14 @@ constexpr long UNSPLIT_BLOCKS = 192, FULL_BLOCKS = 512;
 
 template <int D, int SRC, int PARTS = 1>
 hipError_t launch_decode(const DecodeArgs& p, int num_seqs, hipStream_t stream) {
-  const bool few = p.max_blocks <= (SRC == PAGES_FP8 ? 8 : 4);
+  const bool few = p.max_blocks <= (byte_pages(SRC) ? 8 : 4);
   const long blocks = (long)num_seqs * p.Hkv;
   if (p.n_splits == 1 && blocks >= UNSPLIT_BLOCKS && blocks < FULL_BLOCKS) {
     launch_decode_waves<D, SRC, PARTS, 2 * WAVES>(p, num_seqs, stream);
   } else if (few && p.n_splits == 1 && blocks >= ONE_WAVE_BLOCKS) {
     launch_decode_waves<D, SRC, PARTS, 1>(p, num_seqs, stream);
   } else {
-    if constexpr (SRC == PAGES_FP8) {
+    if constexpr (byte_pages(SRC)) {
       if (p.n_splits <= 2 && blocks < MOST_DEEP_BLOCKS)
         launch_decode_waves<D, SRC, PARTS, 2 * WAVES>(p, num_seqs, stream);
       else
@@ -1098,7 +1176,7 @@ hipError_t launch_decode(const DecodeArgs& p, int num_seqs, hipStream_t stream) 
   HIP_CHECK_KERNEL();
   if (p.n_splits > 1) {
     const long sh = (long)num_seqs * p.H;
-    hipLaunchKernelGGL((paged_attention_reduce_kernel<D, WAVES, PARTS>),
+    hipLaunchKernelGGL((paged_attention_reduce_kernel<D, WAVES, PARTS, SRC == PAGES_FP8S ? PAGES_FP8S : PAGES_REG>),
                        dim3((unsigned)((sh + 3) / 4)), dim3(256), 0, stream, p, sh);
     HIP_CHECK_KERNEL();
   }

@@ -116,7 +116,14 @@ def reshape_and_cache(
     k_cache: torch.Tensor,  # [num_blocks, num_kv_heads, block_size, head_dim]
     v_cache: torch.Tensor,
     slot_mapping: torch.Tensor,  # [num_tokens] int64/int32
+    k_scale: Optional[torch.Tensor] = None,  # [num_blocks, num_kv_heads] E8M0
+    v_scale: Optional[torch.Tensor] = None,
 ) -> None:
+    if k_scale is not None or v_scale is not None:
+        check_scaled_pages(k_cache, v_cache, k_scale, v_scale)
+        write_scaled_pages(k, k_cache, k_scale, slot_mapping)
+        write_scaled_pages(v, v_cache, v_scale, slot_mapping)
+        return
     block_size = k_cache.shape[2]
     slots = slot_mapping.long()
     blk = slots // block_size
@@ -127,6 +134,59 @@ def reshape_and_cache(
     v_cache[blk, :, off] = v.to(v_cache.dtype)
 
 
+#: largest E4M3 number; exponent byte (E8M0) of the smallest scale that is written
+E4M3_MAX = 448.0
+LEAST_SCALE = 27
+
+
+def check_scaled_pages(k_cache, v_cache, k_scale, v_scale) -> None:
+    """What the block-scaled forms are given; pages of any size on the CPU."""
+    if k_scale is None or v_scale is None:
+        raise RuntimeError("scaled pages: k_scale and v_scale go together")
+    for c in (k_cache, v_cache):
+        if c.dtype != torch.float8_e4m3fn or c.dim() != 4 or c.shape != k_cache.shape:
+            raise RuntimeError(
+                "scaled pages: float8_e4m3fn [pages, kv_heads, block, D] expected"
+            )
+    for s in (k_scale, v_scale):
+        if s.dtype != torch.float8_e8m0fnu or s.shape != k_cache.shape[:2]:
+            raise RuntimeError("scaled pages: scales float8_e8m0fnu [pages, kv_heads]")
+
+
+def scaled_pages(cache: torch.Tensor, scale: torch.Tensor) -> torch.Tensor:
+    """The values [pages, kv_heads, block, D] that a block-scaled cache holds, in fp32."""
+    return torch.ldexp(cache.float(), (scale.view(torch.uint8).int() - 127)[..., None, None])
+
+
+def write_scaled_pages(x, cache, scale, slot_mapping) -> None:
+    """New rows x [T, kv_heads, D] into E4M3 pages under one power of two per page and
+    head: the least, 2^-100 at least, that brings the new rows' largest finite value to
+    448 or below, or the page's own where that is larger and the page's first row is
+    not among the new ones. The page's other rows follow a larger scale."""
+    block = cache.shape[2]
+    rows_of = {}
+    for t, slot in enumerate(slot_mapping[: x.shape[0]].tolist()):
+        if 0 <= slot < cache.shape[0] * block:
+            rows_of.setdefault(slot // block, {})[slot % block] = t
+    exponents = scale.view(torch.uint8)
+    for page, rows in rows_of.items():
+        offs, toks = list(rows), list(rows.values())
+        new = x[toks].float().transpose(0, 1)  # [kv, n, D]
+        m, e = torch.frexp(torch.where(new.isfinite(), new.abs(), 0.0).amax(dim=(1, 2)))
+        need = torch.where(m <= 0.875, e - 9, e - 8) + 127
+        need = torch.where(m > 0, need, LEAST_SCALE).clamp(min=LEAST_SCALE)
+        now = need
+        if 0 not in rows:
+            raw = exponents[page].int()
+            old = torch.where(raw == 255, 0, raw)
+            now = torch.maximum(old, need)
+            by = torch.where(raw == 255, -1000, old - now)[:, None, None]
+            cache[page] = torch.ldexp(cache[page].float(), by).to(cache.dtype)
+        coded = torch.ldexp(new, (127 - now)[:, None, None]).clamp(-E4M3_MAX, E4M3_MAX)
+        cache[page][:, offs] = coded.to(cache.dtype)
+        exponents[page] = now.to(torch.uint8)
+
+
 def paged_attention_decode(
     q: torch.Tensor,  # [num_seqs, num_heads, head_dim]
     k_cache: torch.Tensor,  # [num_blocks, num_kv_heads, block_size, head_dim]
@@ -135,7 +195,12 @@ def paged_attention_decode(
     context_lens: torch.Tensor,  # [num_seqs] int32 — includes current token
     scale: float,
     window: int = 0,
+    k_scale: Optional[torch.Tensor] = None,  # [num_blocks, num_kv_heads] E8M0
+    v_scale: Optional[torch.Tensor] = None,
 ) -> torch.Tensor:
+    if k_scale is not None or v_scale is not None:
+        check_scaled_pages(k_cache, v_cache, k_scale, v_scale)
+        k_cache, v_cache = scaled_pages(k_cache, k_scale), scaled_pages(v_cache, v_scale)
     num_seqs, num_heads, head_dim = q.shape
     num_kv_heads = k_cache.shape[1]
     block_size = k_cache.shape[2]
@@ -212,9 +277,14 @@ def context_attention_varlen(
     context_lens: torch.Tensor,  # [num_seqs] total context (incl. new tokens)
     scale: float,
     window: int = 0,
+    k_scale: Optional[torch.Tensor] = None,  # [num_blocks, num_kv_heads] E8M0
+    v_scale: Optional[torch.Tensor] = None,
 ) -> torch.Tensor:
     """Prefill attention against the paged cache (supports chunked prefill:
     new tokens attend to all cached tokens before them, causally)."""
+    if k_scale is not None or v_scale is not None:
+        check_scaled_pages(k_cache, v_cache, k_scale, v_scale)
+        k_cache, v_cache = scaled_pages(k_cache, k_scale), scaled_pages(v_cache, v_scale)
     num_heads = q.shape[1]
     num_kv_heads = k_cache.shape[1]
     head_dim = q.shape[2]
@@ -1122,3 +1192,54 @@ def advance_decode(
     slots[:n] = tables[:n].gather(1, page[:, None])[:, 0] * block + (pos % block).int()
     if seeds is not None:
         seeds[:n] += seed_step
+
+
+def build_paged_batch(
+    pages, page_starts, computed_lens, new_lens, num_tokens: int, max_blocks: int,
+    block_size: int,
+):
+    vectors = (pages, page_starts, computed_lens, new_lens)
+    if any(
+        t.dtype != torch.int32 or t.dim() != 1 or not t.is_contiguous()
+        or t.device != pages.device for t in vectors
+    ):
+        raise RuntimeError("build_paged_batch: dense int32 vectors of one device expected")
+    S = new_lens.shape[0]
+    if page_starts.shape[0] != S + 1 or computed_lens.shape[0] != S:
+        raise RuntimeError(
+            "build_paged_batch: page_starts [S + 1], computed_lens [S] and new_lens [S]"
+        )
+    if (
+        not 0 <= num_tokens < (1 << 31) - 1024 or max_blocks < 0
+        or not 1 <= block_size < 1 << 31 or S * max_blocks >= 1 << 31
+    ):
+        raise RuntimeError("build_paged_batch: sizes out of range")
+    P = pages.shape[0]
+    if P == 0:  # nothing is read from it
+        pages = pages.new_zeros(1)
+    first = page_starts.long()[:-1].clamp(0, P)
+    count = page_starts.long()[1:].clamp(0, P).maximum(first) - first
+    computed, fresh = computed_lens.long().clamp(min=0), new_lens.long().clamp(min=0)
+    ends = torch.cumsum(fresh, 0)
+    begins = ends - fresh
+    t = torch.arange(num_tokens, device=pages.device)
+    seq = torch.searchsorted(ends, t, right=True)
+    real = seq < S
+    ctx = computed + fresh
+    pos = slot = torch.zeros_like(t)
+    if S:
+        row = seq.clamp(max=S - 1)
+        pos = torch.where(real, computed[row] + t - begins[row], 0)
+        held = real & (pos // block_size < count[row])
+        at = torch.where(held, first[row] + pos // block_size, 0)
+        slot = pages[at].long() * block_size + pos % block_size
+        real = held & (slot >= 0) & (slot < 1 << 31)
+    col = torch.arange(max_blocks, device=pages.device)
+    full = col < torch.minimum(-(-ctx // block_size), count)[:, None]
+    tables = torch.where(full, pages[torch.where(full, first[:, None] + col, 0)], 0)
+    i32 = torch.int32
+    cu = torch.cat([ends.new_zeros(1), ends]).clamp(max=num_tokens)
+    return (
+        pos, torch.where(real, slot, -1).to(i32), cu.to(i32), tables.to(i32),
+        ctx.clamp(max=(1 << 31) - 1).to(i32), torch.where(seq < S, seq, -1).to(i32),
+    )

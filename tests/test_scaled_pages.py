@@ -1,0 +1,554 @@
+"""The block-scaled E4M3 cache: batch tables, writes, decode and chunk attention
+against plain forms in 64 bits written here from the definitions.
+
+Whole numbers, bytes and scales have to be equal. Attention's outputs may be off by
+
+- their own rounding, 2^-8 of the value (bf16);
+- scores: D products summed in fp32, (D + 2) 2^-24 of the largest sum M of their sizes
+  (scaled), which moves a weight by that factor above and the denominator below it, and
+  2^-22 of the exponential: twice ((D + 2) 2^-24 M + 2^-22);
+- the sums over L keys and their splits in fp32: (L + 64) 2^-24;
+- chunks: weights rounded to bf16 ahead of their product, 2^-8;
+
+all but the first of the sum of the weighted values' sizes; and weights below 2^-126 of
+the largest may be lost (fp32's normal range), L 2^-126 of the largest value.
+"""
+
+import math
+
+import pytest
+import torch
+
+from kserve_amd import ops
+
+PAGE = 16
+E4M3 = torch.float8_e4m3fn
+E8M0 = torch.float8_e8m0fnu
+
+
+def devices():
+    return ["cpu", pytest.param("cuda", marks=pytest.mark.gpu)]
+
+
+def byte_values():
+    """What the 256 E4M3 bytes stand for, in 64 bits."""
+    v = []
+    for b in range(256):
+        e, m = b >> 3 & 15, b & 7
+        x = (8 + m) * 2.0 ** (e - 10) if e else m * 2.0**-9
+        v.append(math.nan if b & 127 == 127 else -x if b & 128 else x)
+    return torch.tensor(v, dtype=torch.float64)
+
+
+VALUES = byte_values()
+
+
+def nearest_bytes(x):
+    """E4M3 bytes nearest to x (64 bits; NaN stays, larger ones become 448), ties to the
+    even byte: by distance to all of them."""
+    x = x.double()
+    size = x.abs().clamp(max=448.0).reshape(-1)
+    pos = VALUES[:127]
+    hi = torch.searchsorted(pos, size).clamp(max=126)
+    lo = (hi - 1).clamp(min=0)
+    dl, dh = size - pos[lo], pos[hi] - size
+    pick = torch.where(dl < dh, lo, torch.where(dh < dl, hi, torch.where(lo % 2 == 0, lo, hi)))
+    pick = torch.where(x.reshape(-1).isnan(), 127, pick)
+    return (pick + 128 * torch.signbit(x).reshape(-1)).view(x.shape).to(torch.uint8)
+
+
+def held(cache, scale):
+    """A cache's values in 64 bits."""
+    e = scale.view(torch.uint8).cpu().double() - 127
+    return VALUES[cache.view(torch.uint8).cpu().long()] * torch.exp2(e)[..., None, None]
+
+
+def written(x, cache, scale, slots):
+    """(bytes, exponent bytes) after the rows x are written: the definition, page by page."""
+    codes, exps = cache.view(torch.uint8).cpu().clone(), scale.view(torch.uint8).cpu().clone()
+    block = cache.shape[2]
+    pages = {}
+    for t, s in enumerate(slots.tolist()):
+        if 0 <= s < cache.shape[0] * block:
+            pages.setdefault(s // block, {})[s % block] = x[t].cpu().double()
+    for page, rows in pages.items():
+        for h in range(cache.shape[1]):
+            new = torch.stack([r[h] for r in rows.values()])
+            top = float(new[new.isfinite()].abs().max()) if new.isfinite().any() else 0.0
+            e = -100
+            while top > 448 * 2.0**e:
+                e += 1
+            now = e + 127
+            if 0 not in rows:
+                old = int(exps[page, h])
+                now = max(now, 0 if old == 255 else old)
+                factor = 0.0 if old == 255 else 2.0 ** (old - now)
+                if now != old:
+                    codes[page, h] = nearest_bytes(VALUES[codes[page, h].long()] * factor)
+            for o, r in rows.items():
+                codes[page, h, o] = nearest_bytes(r[h] * 2.0 ** (127 - now))
+            exps[page, h] = now
+    return codes, exps
+
+
+def same_bytes(got, want):
+    """Equal, any not-a-number for another."""
+    got = got.view(torch.uint8).cpu()
+    nan = (got & 127) == 127
+    assert torch.equal(nan, (want & 127) == 127)
+    # zeros keep their sign
+    assert torch.equal(got[~nan], want[~nan])
+
+
+def make_cache(pages, kv, D, seed, spread=3.0):
+    g = torch.Generator().manual_seed(seed)
+    codes = torch.randint(0, 256, (pages, kv, PAGE, D), generator=g, dtype=torch.int32)
+    codes = torch.where(codes % 128 == 127, 0, codes).to(torch.uint8)
+    exps = (118 + spread * torch.randn((pages, kv), generator=g)).round().clamp(90, 140)
+    return codes.view(E4M3), exps.to(torch.uint8).view(E8M0)
+
+
+class TestWrite:
+    def check(self, dev, k, v, kc, vc, ks, vs, slots):
+        want = [written(x, c, s, slots) for x, c, s in ((k, kc, ks), (v, vc, vs))]
+        dv = [t.to(dev) for t in (kc, vc)] + [t.view(torch.uint8).to(dev).view(E8M0) for t in (ks, vs)]
+        ops.reshape_and_cache(
+            k if k.device.type == dev else k.to(dev), v if v.device.type == dev else v.to(dev),
+            dv[0], dv[1], slots.to(dev), k_scale=dv[2], v_scale=dv[3],
+        )
+        for i in range(2):
+            same_bytes(dv[i], want[i][0])
+            assert torch.equal(dv[2 + i].view(torch.uint8).cpu(), want[i][1])
+        return dv
+
+    def rows(self, T, kv, D, seed, dev, pad=0):
+        """k and v as views into wider rows (pad more elements a row)."""
+        g = torch.Generator().manual_seed(seed)
+        qkv = torch.randn((T, 4 * kv * D + pad), generator=g)
+        qkv *= torch.exp(2 * torch.randn((T, 1), generator=g))
+        qkv = qkv.to(torch.bfloat16).to(dev)
+        k = qkv[:, kv * D : 2 * kv * D].view(T, kv, D) if pad == 0 else torch.as_strided(
+            qkv, (T, kv, D), (qkv.stride(0), D, 1), kv * D + pad % 8
+        )
+        v = torch.as_strided(qkv, (T, kv, D), (qkv.stride(0), D, 1), 2 * kv * D + pad % 8)
+        return k, v
+
+    @pytest.mark.parametrize("dev", devices())
+    @pytest.mark.parametrize("kv, D", [(1, 64), (8, 128), (3, 128), (9, 64)])
+    @pytest.mark.parametrize("T, first, pad", [(1, 0, 0), (1, 5, 0), (37, 0, 8), (16, 16, 3), (50, 9, 1)])
+    def test_runs_of_slots(self, dev, kv, D, T, first, pad):
+        """Tokens of one sequence, aligned and not, whole and part pages."""
+        kc, ks = make_cache(7, kv, D, 1)
+        vc, vs = make_cache(7, kv, D, 2)
+        k, v = self.rows(T, kv, D, 3, dev, pad)
+        table = torch.tensor([4, 1, 6, 2])
+        pos = torch.arange(first, first + T)
+        slots = (table[pos // PAGE] * PAGE + pos % PAGE).int()
+        self.check(dev, k, v, kc, vc, ks, vs, slots)
+
+    @pytest.mark.parametrize("dev", devices())
+    @pytest.mark.parametrize("T", [3, 100, 1500])
+    def test_any_order(self, dev, T):
+        """Slots in any order, some twice, some out of range: the page's rows are found
+        wherever they stand, and the later of two rows stays."""
+        g = torch.Generator().manual_seed(T)
+        kc, ks = make_cache(40, 2, 64, 4)
+        vc, vs = make_cache(40, 2, 64, 5)
+        k, v = self.rows(T, 2, 64, 6, dev)
+        slots = torch.randint(-20, 40 * PAGE + 20, (T,), generator=g, dtype=torch.int32)
+        if T == 3:
+            slots = torch.tensor([85, 40, 85], dtype=torch.int32)
+        self.check(dev, k, v, kc, vc, ks, vs, slots)
+
+    @pytest.mark.parametrize("dev", devices())
+    def test_unusual_values(self, dev):
+        """Infinities, not-a-numbers, zeros, the type's extremes and its subnormals."""
+        inf, nan = math.inf, math.nan
+        kc, ks = make_cache(12, 1, 64, 7)
+        ks.view(torch.uint8)[3:6] = 255  # pages that hold nothing yet
+        ks.view(torch.uint8)[6:9] = 0
+        special = [
+            [0.0], [inf], [-inf, 1.0], [nan, 2.0], [nan], [3.3895e38], [448.0, 449.0], [450.0],
+            [1e-30, 1e-38], [9.2e-41], [2.0**-100 * 448], [2.0**-101 * 448, inf],
+        ]
+        k = torch.stack([torch.tensor((s * 64)[:64]) for s in special])
+        k = k.to(torch.bfloat16).view(12, 1, 64)
+        for off in (0, 7):
+            slots = torch.arange(12, dtype=torch.int32) * PAGE + off
+            self.check(dev, k, -k, kc, kc.clone(), ks, ks.clone(), slots)
+
+    @pytest.mark.parametrize("dev", devices())
+    def test_growing_page(self, dev):
+        """A page filled token by token, each larger than the one before, holds what a
+        page written at once holds, but for numbers that become subnormal on the way."""
+        g = torch.Generator().manual_seed(11)
+        k = torch.randn((PAGE, 2, 64), generator=g) * torch.exp2(torch.arange(16) / 4)[:, None, None]
+        k = (k.sign() * k.abs().clamp(min=0.25)).to(torch.bfloat16).to(dev)
+        one, two = [[t.to(dev) for t in make_cache(3, 2, 64, 8)] for _ in range(2)]
+        spare = [t.clone() for t in one]
+        ops.reshape_and_cache(k, k, one[0], spare[0], torch.arange(32, 48, dtype=torch.int32, device=dev),
+                              k_scale=one[1], v_scale=spare[1])
+        for i in range(PAGE):
+            ops.reshape_and_cache(k[i : i + 1], k[i : i + 1], two[0], spare[0],
+                                  torch.tensor([32 + i], dtype=torch.int32, device=dev),
+                                  k_scale=two[1], v_scale=spare[1])
+        assert torch.equal(one[1].view(torch.uint8), two[1].view(torch.uint8))
+        assert torch.equal(one[0].view(torch.uint8), two[0].view(torch.uint8))
+        assert torch.equal(two[0].view(torch.uint8), spare[0].view(torch.uint8))
+
+    @pytest.mark.gpu
+    def test_repeats_bitwise(self):
+        """The same call twice leaves the same bytes."""
+        k, v = self.rows(300, 4, 128, 12, "cuda")
+        g = torch.Generator().manual_seed(13)
+        slots = torch.randperm(64 * PAGE, generator=g)[:300].int()
+        outs = []
+        for _ in range(2):
+            kc, ks = make_cache(64, 4, 128, 14)
+            vc, vs = make_cache(64, 4, 128, 15)
+            outs.append(self.check("cuda", k, v, kc, vc, ks, vs, slots))
+        for a, b in zip(*outs):
+            assert torch.equal(a.view(torch.uint8), b.view(torch.uint8))
+
+
+def attention_case(lens, new, heads, kv, D, seed, window=0, spread=3.0):
+    """A cache whose pages stand in any order, with bytes that are not numbers behind
+    every context; queries for the last `new` tokens of each."""
+    g = torch.Generator().manual_seed(seed)
+    counts = [-(-n // PAGE) for n in lens]
+    pages = sum(counts) + 1
+    kc, ks = make_cache(pages, kv, D, seed + 1, spread)
+    vc, vs = make_cache(pages, kv, D, seed + 2, spread)
+    ids = torch.randperm(pages - 1, generator=g) + 1
+    width = max(counts + [1]) + 1
+    table = torch.zeros((len(lens), width), dtype=torch.int32)
+    at = 0
+    for i, c in enumerate(counts):
+        table[i, :c] = ids[at : at + c]
+        at += c
+        if lens[i] % PAGE:
+            for cache in (kc, vc):
+                cache.view(torch.uint8)[table[i, c - 1], :, lens[i] % PAGE :] = 0x7F
+    T = sum(new)
+    q = (4 * torch.randn((T, heads, D), generator=g)).to(torch.bfloat16)
+    cu = torch.tensor([0] + list(torch.tensor(new).cumsum(0)), dtype=torch.int32)
+    return dict(
+        q=q, kc=kc, vc=vc, ks=ks, vs=vs, table=table, cu=cu,
+        ctx=torch.tensor(lens, dtype=torch.int32), window=window, scale=D**-0.5,
+    )
+
+
+def attention_oracle(c):
+    """(outputs, what they may be off by without a rounding of the weights, sums of the
+    weighted values' sizes), in 64 bits."""
+    q = c["q"].double()
+    T, H, D = q.shape
+    k, v = held(c["kc"], c["ks"]), held(c["vc"], c["vs"])
+    kv = k.shape[1]
+    out, off, size = (torch.zeros((T, H, D), dtype=torch.float64) for _ in range(3))
+    for i, L in enumerate(c["ctx"].tolist()):
+        a, b = int(c["cu"][i]), int(c["cu"][i + 1])
+        if a == b or L == 0:
+            continue
+        rows = c["table"][i, : -(-L // PAGE)].long()
+        pos = torch.arange(L - (b - a), L)
+        key = torch.arange(L)
+        hid = key > pos[:, None]
+        if c["window"]:
+            hid |= key <= pos[:, None] - c["window"]
+        for h in range(H):
+            kk = k[rows, h // (H // kv)].reshape(-1, D)[:L]
+            vv = v[rows, h // (H // kv)].reshape(-1, D)[:L]
+            s = (q[a:b, h] @ kk.T) * c["scale"]
+            M = ((q[a:b, h].abs() @ kk.abs().T) * abs(c["scale"])).masked_fill(hid, 0).amax(1)
+            w = torch.softmax(s.masked_fill(hid, -math.inf), dim=1)
+            w = torch.where(hid.all(1, keepdim=True), 0.0, w)
+            out[a:b, h], size[a:b, h] = w @ vv, w @ vv.abs()
+            rel = 2 * ((D + 2) * 2.0**-24 * M + 2.0**-22) + (L + 64) * 2.0**-24
+            off[a:b, h] = rel[:, None] * size[a:b, h] + L * 2.0**-126 * vv.abs().max()
+    return out, off + 2.0**-8 * out.abs(), size
+
+
+def on(c, dev):
+    return {n: t.view(torch.uint8).to(dev).view(t.dtype) if torch.is_tensor(t) and t.dtype in (E4M3, E8M0)
+            else t.to(dev) if torch.is_tensor(t) else t for n, t in c.items()}
+
+
+def decode(c, **more):
+    return ops.paged_attention_decode(
+        c["q"], c["kc"], c["vc"], c["table"], c["ctx"], c["scale"], window=c["window"],
+        k_scale=c["ks"], v_scale=c["vs"], **more,
+    )
+
+
+def context(c, longest=None):
+    n = longest or int((c["cu"][1:] - c["cu"][:-1]).max())
+    return ops.context_attention_varlen(
+        c["q"], c["kc"], c["vc"], c["table"], c["cu"], c["ctx"], n, c["scale"],
+        window=c["window"], k_scale=c["ks"], v_scale=c["vs"],
+    )
+
+
+def near(got, c, chunk=False):
+    out, off, size = attention_oracle(c)
+    if chunk:
+        off = off + 2.0**-8 * size
+    assert got.dtype == torch.bfloat16
+    far = (got.double().cpu() - out).abs() - off
+    assert not got.isnan().any() and float(far.max()) <= 0, float(far.max())
+
+
+class TestDecode:
+    @pytest.mark.parametrize("dev", devices())
+    @pytest.mark.parametrize("D", [64, 128])
+    @pytest.mark.parametrize("heads, kv", [(1, 1), (8, 8), (6, 3), (12, 4), (8, 2), (5, 1), (12, 2), (14, 2), (64, 8)])
+    def test_groups(self, dev, D, heads, kv):
+        c = attention_case([1, 16, 17, 33, 95, 160], [1] * 6, heads, kv, D, 20)
+        near(decode(on(c, dev)), c)
+
+    @pytest.mark.parametrize("dev", devices())
+    @pytest.mark.parametrize("window", [1, 15, 16, 40, 1000])
+    def test_windows(self, dev, window):
+        c = attention_case([1, 16, 31, 48, 300], [1] * 5, 8, 2, 64, 30, window)
+        near(decode(on(c, dev)), c)
+
+    @pytest.mark.gpu
+    @pytest.mark.parametrize("D", [64, 128])
+    @pytest.mark.parametrize(
+        "lens, heads, kv",
+        [([5000], 8, 1), ([2047, 1, 640], 16, 2), ([100 + 7 * i for i in range(40)], 32, 8),
+         ([17] * 300, 8, 8), ([30] * 520, 4, 4), ([600] * 70, 8, 8)],
+    )
+    def test_splits_and_waves(self, D, lens, heads, kv):
+        """Contexts in one part and in several, launches of one, two and four waves."""
+        c = attention_case(lens, [1] * len(lens), heads, kv, D, 40)
+        near(decode(on(c, "cuda")), c)
+
+    @pytest.mark.parametrize("dev", devices())
+    def test_extreme_scales(self, dev):
+        """Pages from 2^-90 to 2^13 beside one another."""
+        c = attention_case([100, 64], [1, 1], 4, 2, 128, 50)
+        c["ks"].view(torch.uint8)[::3] = 37
+        c["vs"].view(torch.uint8)[::2] = 140
+        near(decode(on(c, dev)), c)
+
+    @pytest.mark.gpu
+    def test_empty_context_and_out(self):
+        """A sequence without keys gives zeros; `out` is filled and returned."""
+        c = attention_case([40, 1, 20], [1] * 3, 8, 2, 128, 60)
+        c["ctx"][1] = 0
+        d = on(c, "cuda")
+        out = torch.full_like(d["q"], 7.0)
+        assert decode(d, out=out) is out
+        assert not out[1].any()
+        near(out, c)
+
+    @pytest.mark.gpu
+    def test_strided_queries_and_negative_scale(self):
+        c = attention_case([40, 100], [1] * 2, 8, 2, 64, 70)
+        c["scale"] = -c["scale"]
+        d = on(c, "cuda")
+        wide = torch.zeros((2, 12, 64), dtype=torch.bfloat16, device="cuda")
+        wide[:, 2:10] = d["q"]
+        d["q"] = wide[:, 2:10]
+        near(decode(d), c)
+
+    @pytest.mark.gpu
+    def test_ids_outside_the_cache(self):
+        """Table entries and lengths out of range stay inside the cache."""
+        c = attention_case([40, 100], [1] * 2, 8, 2, 128, 80)
+        d = on(c, "cuda")
+        d["table"][0, 1], d["table"][0, 2] = -5, 1 << 30
+        d["ctx"][0] = 1 << 30
+        got = decode(d)
+        c["q"], c["cu"], c["ctx"], c["table"] = c["q"][1:], c["cu"][:2], c["ctx"][1:], c["table"][1:]
+        near(got[1:], c)
+
+
+class TestContext:
+    @pytest.mark.parametrize("dev", devices())
+    @pytest.mark.parametrize("D", [64, 128])
+    @pytest.mark.parametrize("heads, kv", [(1, 1), (6, 2), (8, 2), (7, 1)])
+    def test_chunks(self, dev, D, heads, kv):
+        c = attention_case([1, 16, 50, 129, 200], [1, 16, 3, 70, 33], heads, kv, D, 100)
+        near(context(on(c, dev)), c, True)
+
+    @pytest.mark.parametrize("dev", devices())
+    @pytest.mark.parametrize("window", [1, 16, 60])
+    def test_windows(self, dev, window):
+        c = attention_case([64, 150, 20], [64, 70, 5], 8, 2, 64, 110, window)
+        near(context(on(c, dev)), c, True)
+
+    @pytest.mark.gpu
+    @pytest.mark.parametrize("D", [64, 128])
+    def test_split_keys(self, D):
+        """Few queries behind long contexts: keys in parts, the sums merged."""
+        c = attention_case([3000, 2500], [20, 9], 8, 2, D, 120)
+        near(context(on(c, "cuda")), c, True)
+
+    @pytest.mark.gpu
+    def test_sequences_without_queries(self):
+        c = attention_case([64, 100, 40], [0, 7, 0], 8, 2, 128, 130)
+        near(context(on(c, "cuda")), c, True)
+
+    @pytest.mark.gpu
+    def test_ids_outside_the_cache(self):
+        c = attention_case([40, 100], [9, 30], 8, 2, 128, 140)
+        d = on(c, "cuda")
+        d["table"][0] = torch.tensor([-5, 1 << 30, 3] + [0] * (d["table"].shape[1] - 3))
+        d["ctx"][0] = 1 << 30
+        got = context(d)
+        near(got[9:], dict(c, q=c["q"][9:], cu=c["cu"][1:] - 9, ctx=c["ctx"][1:], table=c["table"][1:]), True)
+
+
+def batch_oracle(lists, computed, new, rows, width, block):
+    pos, slots, seqs, cu = [], [], [], [0]
+    tables = []
+    for s, (pages, c, n) in enumerate(zip(lists, computed, new)):
+        for p in range(c, c + n):
+            pos.append(p)
+            slots.append(pages[p // block] * block + p % block if p // block < len(pages) else -1)
+            seqs.append(s)
+        cu.append(min(cu[-1] + n, rows))
+        full = min(-(-(c + n) // block), len(pages))
+        tables.append((pages[:full] + [0] * width)[:width])
+    fill = max(0, rows - len(pos))
+    return (
+        (pos + [0] * fill)[:rows], (slots + [-1] * fill)[:rows], cu, tables,
+        [c + n for c, n in zip(computed, new)], (seqs + [-1] * fill)[:rows],
+    )
+
+
+class TestBatch:
+    def run(self, dev, lists, computed, new, rows, width, block):
+        starts = [0]
+        for x in lists:
+            starts.append(starts[-1] + len(x))
+
+        def vec(x):
+            return torch.tensor(x, dtype=torch.int32, device=dev)
+
+        got = ops.build_paged_batch(
+            vec([i for x in lists for i in x]), vec(starts), vec(computed), vec(new), rows,
+            width, block,
+        )
+        want = batch_oracle(lists, computed, new, rows, width, block)
+        assert got.positions.dtype == torch.int64
+        assert all(t.dtype == torch.int32 for t in got[1:])
+        assert got.block_tables.shape == (len(lists), width)
+        for g, w in zip(got, want):
+            assert g.device.type == dev and g.tolist() == w
+
+    @pytest.mark.parametrize("dev", devices())
+    @pytest.mark.parametrize("block", [1, 4, 16, 100])
+    @pytest.mark.parametrize(
+        "computed, new, pad",
+        [([0], [1], 0), ([0], [77], 3), ([5, 0, 160], [1, 0, 40], 0), ([0, 0], [0, 0], 0),
+         ([0, 3, 0], [0, 9, 0], 5), ([], [], 4), ([], [], 0)],
+    )
+    def test_small(self, dev, computed, new, pad, block):
+        g = torch.Generator().manual_seed(block)
+        lists = [
+            torch.randint(1, 1000, (-(-(c + n) // block) + i % 2,), generator=g).tolist()
+            for i, (c, n) in enumerate(zip(computed, new))
+        ]
+        width = max([-(-(c + n) // block) for c, n in zip(computed, new)] + [0])
+        self.run(dev, lists, computed, new, sum(new) + pad, width, block)
+
+    @pytest.mark.parametrize("dev", devices())
+    @pytest.mark.parametrize("S", [3, 1023, 1024, 1025, 2500])
+    def test_many_requests(self, dev, S):
+        """Past a block's chunk of lengths and of tokens."""
+        g = torch.Generator().manual_seed(S)
+        computed = torch.randint(0, 60, (S,), generator=g).tolist()
+        new = torch.randint(0, 4 if S > 3 else 3000, (S,), generator=g).tolist()
+        lists = [
+            torch.randint(0, 1 << 20, (-(-(c + n) // PAGE),), generator=g).tolist()
+            for c, n in zip(computed, new)
+        ]
+        width = max(len(x) for x in lists)
+        self.run(dev, lists, computed, new, sum(new) + 11, width, PAGE)
+
+    @pytest.mark.parametrize("dev", devices())
+    def test_short_lists_and_rows(self, dev):
+        """Tokens past their request's pages have no slot; rows and tables that are too
+        short hold the first."""
+        self.run(dev, [[7], [9, 8, 5]], [10, 0], [20, 40], 50, 2, PAGE)
+
+    @pytest.mark.parametrize("dev", devices())
+    def test_starts_out_of_range(self, dev):
+        """Page lists that point outside stay inside."""
+
+        def vec(x):
+            return torch.tensor(x, dtype=torch.int32, device=dev)
+
+        got = ops.build_paged_batch(vec([3, 4]), vec([-9, 1, 900]), vec([0, 0]), vec([20, 30]), 50, 3, PAGE)
+        assert got.block_tables.tolist() == [[3, 0, 0], [4, 0, 0]]
+        assert got.slot_mapping.tolist() == (
+            list(range(48, 64)) + [-1] * 4 + list(range(64, 80)) + [-1] * 14
+        )
+
+
+class TestRefusals:
+    """The same calls are refused on both sides."""
+
+    @pytest.mark.parametrize("dev", devices())
+    def test_batch(self, dev):
+        def vec(x, dtype=torch.int32):
+            return torch.tensor(x, dtype=dtype, device=dev)
+
+        good = [vec([1, 2]), vec([0, 2]), vec([0]), vec([20]), 20, 2, PAGE]
+        ops.build_paged_batch(*good)
+        for i, bad in [
+            (0, vec([1, 2], torch.int64)), (1, vec([0])), (1, vec([0, 1, 2])), (2, vec([0, 0])),
+            (3, vec([[20]])), (3, vec([20], torch.int64)), (4, -1), (4, 1 << 31), (5, -1),
+            (5, 1 << 31), (6, 0), (0, vec([1, 1, 2, 2])[::2]),
+        ]:
+            args = list(good)
+            args[i] = bad
+            with pytest.raises(RuntimeError):
+                ops.build_paged_batch(*args)
+
+    @pytest.mark.parametrize("dev", devices())
+    def test_pages(self, dev):
+        c = on(attention_case([20], [1], 4, 2, 64, 200), dev)
+        k = torch.zeros((1, 2, 64), dtype=torch.bfloat16, device=dev)
+        slots = torch.zeros(1, dtype=torch.int32, device=dev)
+        scales = c["ks"].view(torch.uint8)
+        for bad in [
+            dict(ks=None), dict(vs=None), dict(ks=scales), dict(ks=scales[:1].view(E8M0)),
+            dict(vs=scales.float()), dict(vc=c["vc"][:1]), dict(kc=c["kc"].float()),
+        ]:
+            x = dict(c, **bad)
+            with pytest.raises(RuntimeError):
+                decode(x)
+            with pytest.raises(RuntimeError):
+                context(x)
+            with pytest.raises(RuntimeError):
+                ops.reshape_and_cache(k, k, x["kc"], x["vc"], slots, k_scale=x["ks"], v_scale=x["vs"])
+
+    @pytest.mark.gpu
+    def test_kernels_forms(self):
+        """What the kernels do not take: other head sizes, larger groups, other types and
+        devices."""
+        c = on(attention_case([20], [1], 4, 2, 64, 210), "cuda")
+        big = on(attention_case([20], [1], 18, 2, 64, 220), "cuda")
+        with pytest.raises(RuntimeError):
+            decode(big)  # nine heads to a KV head
+        near(context(big), on(big, "cpu"), True)
+        for bad in [
+            dict(q=c["q"].half()), dict(q=c["q"].cpu()), dict(q=c["q"][:, :3]),
+            dict(table=c["table"].long()), dict(table=c["table"][:0]), dict(ctx=c["ctx"].long()),
+            dict(ctx=c["ctx"].cpu()), dict(window=-1), dict(kc=c["kc"][..., :32], vc=c["vc"][..., :32]),
+        ]:
+            with pytest.raises(RuntimeError):
+                decode(dict(c, **bad))
+            with pytest.raises(RuntimeError):
+                context(dict(c, **bad), 1)
+        with pytest.raises(RuntimeError):
+            context(dict(c, cu=c["cu"].long()))
+        k = torch.zeros((2, 2, 64), dtype=torch.bfloat16, device="cuda")
+        slots = torch.zeros(2, dtype=torch.int32, device="cuda")
+        for x, s in [(k, slots[:1]), (k, slots.long()), (k, slots.cpu()), (k.float(), slots), (k[:, :1], slots)]:
+            with pytest.raises(RuntimeError):
+                ops.reshape_and_cache(x, x, c["kc"], c["vc"], s, k_scale=c["ks"], v_scale=c["vs"])
