@@ -34,6 +34,7 @@ MODULES = {
             "kv_cache.hip",
             "attention_decode.hip",
             "attention_prefill.hip",
+            "attention_scaled.hip",
             "sampling.hip",
             "decode_step.hip",
             "paged_batch.hip",

@@ -73,28 +73,3 @@ extern "C" hipError_t ks_paged_attention_decode(
   if (head_dim == 64 && !fp8) return launch_decode<64, PAGES_REG>(p, num_seqs, stream);
   return hipErrorInvalidValue;
 }
-
-extern "C" hipError_t ks_paged_attention_decode_scaled(
-    void* out, const void* q, const void* k_cache, const void* v_cache,
-    const void* k_scale, const void* v_scale, const void* block_tables,
-    const void* context_lens, float scale, int num_seqs, int num_heads, int num_kv_heads,
-    int head_dim, int max_blocks, int pages, long q_row_stride, int n_splits,
-    void* part_out, void* part_ml, int window, hipStream_t stream) {
-  if (num_kv_heads < 1 || num_heads % num_kv_heads != 0 || pages < 1)
-    return hipErrorInvalidValue;
-  const int group = num_heads / num_kv_heads;
-  if (group < 1 || group > 8) return hipErrorInvalidValue;
-  if (num_seqs == 0) return hipSuccess;
-  if (n_splits < 1 || !part_out || !part_ml) n_splits = 1;
-  const DecodeArgs p{out, q, k_cache, v_cache,
-                     (const int*)block_tables, (const int*)context_lens,
-                     score_scale(scale),
-                     num_heads, num_kv_heads, group, max_blocks, q_row_stride,
-                     n_splits, (float*)part_out, (float*)part_ml, window,
-                     head_dim, head_dim, nullptr, Extra{},
-                     Scales{(const unsigned char*)k_scale, (const unsigned char*)v_scale,
-                            pages}};
-  if (head_dim == 128) return launch_decode<128, PAGES_FP8S>(p, num_seqs, stream);
-  if (head_dim == 64) return launch_decode<64, PAGES_FP8S>(p, num_seqs, stream);
-  return hipErrorInvalidValue;
-}

@@ -1,0 +1,470 @@
+// Paged decode attention over the block-scaled E4M3 cache (bf16 queries, one per
+// sequence): o = sum_j softmax_j(scale q k_j) v_j, where a page's bytes of one KV head
+// stand for code * 2^e.
+//
+// A block takes the query heads of one KV head of one sequence (or of one of several
+// splits of its context); its waves take pairs of pages in turn, each by itself until the
+// sums are merged. Both products run transposed on v_mfma_f32_16x16x32_bf16: S^T = K Q^T
+// has a query head per lane column, and its registers are the B operand of O^T += V^T P^T
+// (contraction index 8 g + j: key 4 g + j of the first page for j < 4, of the second after
+// that). Bytes become bf16 by the scaling conversions, which apply the page's power of two
+// exactly and for nothing.
+//
+// K goes from memory into the product's registers: a contraction may take its columns in
+// any order that both operands share, so a lane takes 16 consecutive bytes of its key's
+// row for two products, and the query is laid out to match. V passes through LDS of the
+// wave's own, to be read back by the transposing loads. Neither has addresses per lane:
+// a page's rows of one head lie together, and whole pages are read. What lies outside the
+// context or the window may be anything: scores there are replaced and rows of V zeroed.
+// Page ids and scales are fetched for 32 pairs at once, a page to a lane.
+//
+// The weights keep 24 bits as three bf16 parts, as in attention_decode.hip: in the 16
+// columns side by side for groups of up to five heads, by a second product for six to
+// eight.
+#include <type_traits>
+
+#include "mfma_attention.h"
+
+namespace {
+
+using namespace mfma_attn;
+
+struct ScaledDecode {
+  void* out;                       // [S, H, D] bf16
+  const short* q;                  // [S, H, D] bf16, row stride sq
+  const unsigned char* k_cache;    // [pages, Hkv, 16, D]
+  const unsigned char* v_cache;
+  Scales s8;
+  const int* block_tables;         // [S, max_blocks]
+  const int* ctx_lens;             // [S]
+  float scale;
+  int H, Hkv, group, max_blocks;
+  long sq;
+  int n_splits;
+  float* part_out;  // [S, H, n_splits, D]
+  float* part_ml;   // [S, H, n_splits, 2]
+  int window;
+};
+
+// keys of sequence s: as many as its table row has at most
+__device__ __forceinline__ int context_of(const ScaledDecode& p, int s) {
+  return min(p.ctx_lens[s], p.max_blocks * PAGE);
+}
+
+// 16-byte chunk that chunk c of staged row r is XORed with: the 16 rows of both pages
+// that half a wave's transposing load brings lie in different banks
+template <int D>
+__device__ __forceinline__ int byte_swz(int r) {
+  if constexpr (D == 128) return ((r >> 1) & 7) ^ (r >> 4 & 1) << 2;
+  else return ((r >> 2) & 3) ^ (r >> 4 & 1) << 1;
+}
+
+// Adds to the first G columns of 16 the ones G and (PARTS 3) 2 G further on.
+template <int G, int PARTS, int N>
+__device__ __forceinline__ void add_parts(f32x4_t (&o)[N]) {
+  auto from = [](float x, auto by) {  // the value `by` columns on
+    return __builtin_bit_cast(
+        float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, x),
+                                           0x120 + 16 - decltype(by)::value, 15, 15, true));
+  };
+#pragma unroll
+  for (int b = 0; b < N; ++b)
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      const float x = o[b][r];
+      float sum = x + from(x, std::integral_constant<int, G>{});
+      if constexpr (PARTS == 3) sum += from(x, std::integral_constant<int, 2 * G>{});
+      o[b][r] = sum;
+    }
+}
+
+constexpr int BATCH = 32;  // pairs whose page ids and scales a wave fetches at once
+
+template <int D, int NW, bool WIDE>  // WIDE: groups of 6 to 8
+__global__ __launch_bounds__(NW * 64, 4) void scaled_decode_kernel(const ScaledDecode p) {
+  constexpr int KC = D / 32;       // contraction chunks of K Q^T
+  constexpr int DB = D / 16;       // 16-column blocks of the output
+  constexpr int ROWS = 2 * PAGE;   // keys of a pair
+  constexpr int TILE = PAGE * D;   // bytes of a page of one head
+  constexpr int NI = D / 64;       // wave-wide 16-byte loads of a page
+  constexpr int LPR = D / 16;      // lanes per row of V as it is loaded
+  constexpr int MERGE = 8 * (D + 4) + 16;  // floats: sums of 8 heads, their m and l
+  constexpr int AREA = MERGE * 4 > 2 * TILE ? MERGE * 4 : 2 * TILE;
+
+  const int kvh = blockIdx.x, s = blockIdx.y, split = blockIdx.z;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int lane = threadIdx.x & 63;
+  const int* bt = p.block_tables + (long)s * p.max_blocks;
+
+  // Lane l of a batch from pair n on: page (l & 1) of pair n + l / 2 * NW. Where a wave's
+  // first pair does not depend on the context, its page ids are on the way before that is
+  // known (entries behind the context are not used).
+  int id = 0;
+  const bool known = p.n_splits == 1 && p.window == 0;
+  if (known) id = bt[min(2 * (wave + (lane >> 1) * NW) + (lane & 1), p.max_blocks - 1)];
+  const int ctx = context_of(p, s);
+  const Range rg = page_range(ctx, p.window, 0, p.n_splits, NW);
+  const int n_lo = split * rg.per + wave;
+  const int n_hi = min((split + 1) * rg.per, rg.pairs);
+  // waves with work, the first at least: the others end here and no barrier waits for them
+  const int nw = min(max(n_hi - split * rg.per, 1), NW);
+  if (split >= rg.splits || wave >= nw) return;
+  const int col = lane & 15, g = lane >> 4;
+  const int G = p.group;
+  const int part = col / G;  // of the weights: high, middle, low
+  const bool used = part < (WIDE ? 2 : 3);
+
+  __shared__ __attribute__((aligned(16))) char lds[NW][AREA];
+
+  unsigned int ks = 0, vs = 0;
+  auto fetch_scales = [&]() {
+    id = min(max(id, 0), p.s8.pages - 1);
+    const long at = (long)id * p.Hkv + kvh;
+    ks = p.s8.k[at];
+    vs = p.s8.v[at];
+  };
+  auto fetch = [&](int n) {
+    id = bt[min(rg.first + 2 * (n + (lane >> 1) * NW) + (lane & 1), rg.last)];
+    fetch_scales();
+  };
+  uint4 kr[2][NI], vr[2][NI];
+  const unsigned int klane = col * D + g * 16, vlane = lane * 16;
+  auto tile = [&](const unsigned char* cache, int i, int h) {
+    const int page = __builtin_amdgcn_readlane(id, (i % BATCH) * 2 + h);
+    const char* at = reinterpret_cast<const char*>(cache) + ((long)page * p.Hkv + kvh) * TILE;
+    // (kept apart from the lanes' 32-bit offsets: joined they are 64 bits of each lane)
+    asm("" : "+s"(at));
+    return at;
+  };
+  auto load_k = [&](int i) {
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const char* from = tile(p.k_cache, i, h);
+#pragma unroll
+      for (int j = 0; j < NI; ++j) kr[h][j] = load16_nt(from + klane + j * 64);
+    }
+  };
+  auto load_v = [&](int i) {
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const char* from = tile(p.v_cache, i, h);
+#pragma unroll
+      for (int j = 0; j < NI; ++j) vr[h][j] = load16_nt(from + vlane + j * 1024);
+    }
+  };
+  if (n_lo < n_hi) {
+    if (known) fetch_scales();
+    else fetch(n_lo);
+    load_k(0);
+    load_v(0);
+  }
+
+  bf16x8_t qf[KC];
+  float c2 = p.scale * LOG2E;
+  {
+    const short flip = c2 < 0.f ? (short)0x8000 : (short)0;  // the scale's sign, exactly
+    const short* qp = p.q + (long)s * p.sq + (long)(kvh * G + col % G) * D + g * 16;
+#pragma unroll
+    for (int c = 0; c < KC; ++c) {
+      short8_t x = *reinterpret_cast<const short8_t*>(qp + (c >> 1) * 64 + (c & 1) * 8);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) x[j] = used ? (short)(x[j] ^ flip) : (short)0;
+      qf[c] = __builtin_bit_cast(bf16x8_t, x);
+    }
+  }
+  c2 = fabsf(c2);
+
+  // Transposing load: lane i of 16 brings key i / 2, columns 8 (i % 2) .. + 7, and
+  // receives column i of eight keys, four of each page.
+  const int vrow = (col >> 3) * PAGE + g * 4 + ((col >> 1) & 3);
+  unsigned int vaddr = vrow * D + byte_swz<D>(vrow) * 16 + (col & 1) * 8;
+  // where a lane's bytes of V go: of the loads with odd h + j half a row of chunks off
+  unsigned int to[2];
+  to[0] = lane / LPR * D + ((lane % LPR) ^ byte_swz<D>(lane / LPR)) * 16;
+  to[1] = to[0] ^ (D / 2);
+
+  const int key_lo = ctx > 0 ? low_of(ctx - 1, p.window, 0) : 0;  // first visible key
+  // Weights are 2^(score c2 - mc); mc follows the largest score once it is passed by 2^8
+  constexpr float ROOM = 8.f;
+  float mc = fmaxf(NO_MAX * c2, -3e38f), l = 0.f;
+  f32x4_t o[DB];
+#pragma unroll
+  for (int b = 0; b < DB; ++b) o[b] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+
+  for (int n = n_lo, i = 0; n < n_hi; n += NW, ++i) {
+    float k2[2], v2[2];
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      k2[h] = page_scale(__builtin_amdgcn_readlane(ks, (i % BATCH) * 2 + h));
+      v2[h] = page_scale(__builtin_amdgcn_readlane(vs, (i % BATCH) * 2 + h));
+    }
+    const bool more = n + NW < n_hi;
+    if (more && (i + 1) % BATCH == 0) fetch(n + NW);
+
+    f32x4_t sc[2];
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      sc[h] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int c = 0; c < KC; ++c) {
+        const uint4 x = kr[h][c >> 1];
+        const uint2 half = c & 1 ? uint2{x.z, x.w} : uint2{x.x, x.y};
+        sc[h] = mfma16x16x32(widen_fp8(half, k2[h]), qf[c], sc[h]);
+      }
+    }
+    if (more) load_k(i + 1);
+    const int key0 = (rg.first + 2 * n) * PAGE;
+    const bool edge = key0 + ROWS > ctx || key0 < key_lo;
+    if (edge) {
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          const int key = key0 + h * PAGE + g * 4 + r;
+          sc[h][r] = key < ctx && key >= key_lo ? sc[h][r] : MASKED;
+        }
+#pragma unroll
+        for (int j = 0; j < NI; ++j) {
+          const int key = key0 + h * PAGE + j * (64 / LPR) + lane / LPR;
+          if (key >= ctx || key < key_lo) vr[h][j] = uint4{0, 0, 0, 0};
+        }
+      }
+    }
+    char* mine = lds[wave];
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+#pragma unroll
+      for (int j = 0; j < NI; ++j)
+        *reinterpret_cast<uint4*>(mine + to[(h + j) & 1] + (h * PAGE + j * (64 / LPR)) * D) =
+            vr[h][j];
+    if (more) load_v(i + 1);
+
+    float mx = fmaxf(fmaxf(fmaxf(sc[0][0], sc[0][1]), fmaxf(sc[0][2], sc[0][3])),
+                     fmaxf(fmaxf(sc[1][0], sc[1][1]), fmaxf(sc[1][2], sc[1][3])));
+    mx = column_max(mx) * c2;
+    if (__any(mx > mc + ROOM)) {
+      const float mn = fmaxf(mc, mx);
+      const float f = __builtin_amdgcn_exp2f(mc - mn);
+      mc = mn;
+      l *= f;
+#pragma unroll
+      for (int b = 0; b < DB; ++b) o[b] *= f;
+    }
+    asm("" : "+v"(vaddr));  // (its eight forms are made here, not kept)
+    bf16x8_t pf, pl;
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const float w = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[h][r], c2, -mc));
+        l += w;
+        const Split3 w3(w);
+        if constexpr (WIDE) {
+          pf[h * 4 + r] = part == 0 ? w3.hi : w3.mid;
+          pl[h * 4 + r] = part == 0 ? w3.lo : (__bf16)0.f;
+        } else {
+          pf[h * 4 + r] = part == 0 ? w3.hi : part == 1 ? w3.mid : w3.lo;
+        }
+      }
+#pragma unroll
+    for (int b = 0; b < DB; ++b) {
+      typedef int i2_t __attribute__((ext_vector_type(2)));
+      typedef __attribute__((address_space(3))) i2_t lds2_t;
+      const char* a0 = mine + (vaddr ^ b * 16);
+      const bf16x8_t a = widen_pages(
+          __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr8_b64_v2i32((lds2_t*)a0)),
+          v2[0], v2[1]);
+      o[b] = mfma16x16x32(a, pf, o[b]);
+      if constexpr (WIDE) o[b] = mfma16x16x32(a, pl, o[b]);
+    }
+  }
+
+  // ---- merge: the parts of the weights, then the waves ----
+  l = column_sum(l);
+  float* mo = reinterpret_cast<float*>(lds[wave]);  // [8][D + 4], then m and l
+  float* mm = mo + 8 * (D + 4);
+  constexpr int PARTS = WIDE ? 2 : 3;
+  if constexpr (WIDE) {
+    if (G == 8) add_parts<8, PARTS>(o);
+    else if (G == 7) add_parts<7, PARTS>(o);
+    else add_parts<6, PARTS>(o);
+  } else {
+    if (G == 4) add_parts<4, PARTS>(o);
+    else if (G == 1) add_parts<1, PARTS>(o);
+    else if (G == 2) add_parts<2, PARTS>(o);
+    else if (G == 3) add_parts<3, PARTS>(o);
+    else add_parts<5, PARTS>(o);
+  }
+  if (col < G) {
+#pragma unroll
+    for (int b = 0; b < DB; ++b)
+      *reinterpret_cast<f32x4_t*>(mo + col * (D + 4) + b * 16 + g * 4) = o[b];
+  }
+  if (lane < G) {
+    mm[lane] = mc;
+    mm[8 + lane] = l;
+  }
+  __syncthreads();
+  constexpr int WF = AREA / 4;  // floats between the waves' areas
+  const float* all = reinterpret_cast<const float*>(lds);
+  for (int i = threadIdx.x; i < G * (D / 4); i += nw * 64) {
+    const int h = i / (D / 4), d = i % (D / 4) * 4;
+    float top = all[8 * (D + 4) + h];
+#pragma unroll
+    for (int w = 1; w < NW; ++w)
+      if (w < nw) top = fmaxf(top, all[w * WF + 8 * (D + 4) + h]);
+    float sum = 0.f;
+    f32x4_t acc = f32x4_t{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int w = 0; w < NW; ++w) {
+      if (w >= nw) continue;
+      const float* a = all + w * WF;
+      const float f = __builtin_amdgcn_exp2f(a[8 * (D + 4) + h] - top);
+      sum += f * a[8 * (D + 4) + 8 + h];
+      acc += f * *reinterpret_cast<const f32x4_t*>(a + h * (D + 4) + d);
+    }
+    const int head = kvh * G + h;
+    if (rg.splits == 1) {
+      store4(p.out, ((long)s * p.H + head) * D + d, acc * (sum > 0.f ? 1.f / sum : 0.f), 0);
+    } else {
+      const long at = ((long)s * p.H + head) * p.n_splits + split;
+      *reinterpret_cast<f32x4_t*>(p.part_out + at * D + d) = acc;
+      if (d == 0) {
+        p.part_ml[at * 2] = top;
+        p.part_ml[at * 2 + 1] = sum;
+      }
+    }
+  }
+}
+
+// Adds the splits of a (sequence, head): four waves take every fourth one, in order.
+// Sequences that one split covers are done.
+template <int D>
+__global__ __launch_bounds__(256) void scaled_decode_reduce_kernel(const ScaledDecode p,
+                                                                   const int waves) {
+  constexpr int ACC = D / 64;
+  const int h = blockIdx.x, s = blockIdx.y;
+  const Range rg = page_range(context_of(p, s), p.window, 0, p.n_splits, waves);
+  if (rg.splits == 1) return;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const long sh = (long)s * p.H + h;
+  const float* ml = p.part_ml + sh * p.n_splits * 2;
+  float m = -3.4e38f;
+  for (int sp = lane; sp < rg.splits; sp += 64) m = fmaxf(m, ml[sp * 2]);
+  m = wave_reduce_max(m);
+  float l = 0.f, acc[ACC];
+#pragma unroll
+  for (int a = 0; a < ACC; ++a) acc[a] = 0.f;
+#pragma unroll 4
+  for (int sp = wave; sp < rg.splits; sp += 4) {
+    const float w = __builtin_amdgcn_exp2f(ml[sp * 2] - m);
+    l += w * ml[sp * 2 + 1];
+    const float* po = p.part_out + (sh * p.n_splits + sp) * D + lane * ACC;
+#pragma unroll
+    for (int a = 0; a < ACC; ++a) acc[a] += w * po[a];
+  }
+  __shared__ float sums[4][D + 1];
+#pragma unroll
+  for (int a = 0; a < ACC; ++a) sums[wave][lane * ACC + a] = acc[a];
+  if (lane == 0) sums[wave][D] = l;
+  __syncthreads();
+  if (threadIdx.x >= D) return;
+  const int d = threadIdx.x;
+  const float all = sums[0][D] + sums[1][D] + sums[2][D] + sums[3][D];
+  const float x = sums[0][d] + sums[1][d] + sums[2][d] + sums[3][d];
+  reinterpret_cast<short*>(p.out)[sh * D + d] =
+      float_to_bf16_bits(x * (all > 0.f ? 1.f / all : 0.f));
+}
+
+// Waves that share a context, 4 or 8, and its splits.
+//
+// From UNIT_BLOCKS blocks on, one to a compute unit, four waves and no splits (us, 4 x 1 / 8
+// x 1 / 4 waves x 2 splits, 8 KV heads of 128: 32 sequences of 1500 +- 60% 26.9 / 25.9 /
+// 29.9, 64 of 600 +- 50% 21.3 / 21.9 / 27.4, 96 of 3000 +- 60% 118 / 124 / 125, 256 of 100
+// 20 / 25 / 31, of 2048 +- 60% 199 / 197 / 218). Below, splits make up that many blocks (1
+// of 131071 under groups of eight 81 / 52 / 53 with 16, 32 and 64, of 7000 14.5 / 13.2 /
+// 15.1; 8 of 1500 17.5 / 14.4 / 14.7 with 2, 4 and 8), unless eight waves take a table in
+// SHORT pairs each, which spares the launch that merges (1 of 560 10.2, as 4 x 4 12.9; 1 of
+// 2000 20.1 and 12.3 as 4 x 16). Waves without a pair end at once (1000 of 16 tokens 42 ->
+// 23).
+struct Shape {
+  int waves, splits;
+};
+constexpr long UNIT_BLOCKS = 256, SHORT = 4;
+Shape decode_shape(long seqs, long kv_heads, long max_blocks) {
+  const long blocks = seqs * kv_heads;
+  if (blocks <= 0 || blocks >= UNIT_BLOCKS) return {4, 1};
+  const long pairs = (max_blocks + 1) / 2;
+  const long splits = (UNIT_BLOCKS + blocks / 2) / blocks;
+  if (pairs <= 8 * SHORT || splits == 1) return {8, 1};
+  const long most = (pairs + 3) / 4;  // a pair for every wave
+  return {4, (int)(splits < most ? splits : most)};
+}
+
+template <int D, int NW>
+void launch_waves(const ScaledDecode& p, dim3 grid, hipStream_t stream) {
+  if (3 * p.group <= 16)
+    hipLaunchKernelGGL((scaled_decode_kernel<D, NW, false>), grid, dim3(NW * 64), 0, stream, p);
+  else
+    hipLaunchKernelGGL((scaled_decode_kernel<D, NW, true>), grid, dim3(NW * 64), 0, stream, p);
+}
+
+template <int D>
+hipError_t launch_scaled(const ScaledDecode& p, int seqs, int waves, hipStream_t stream) {
+  const dim3 grid(p.Hkv, seqs, p.n_splits);
+  if (waves == 8) launch_waves<D, 8>(p, grid, stream);
+  else launch_waves<D, 4>(p, grid, stream);
+  HIP_CHECK_KERNEL();
+  if (p.n_splits > 1) {
+    hipLaunchKernelGGL((scaled_decode_reduce_kernel<D>), dim3(p.H, seqs), dim3(256), 0,
+                       stream, p, waves);
+    HIP_CHECK_KERNEL();
+  }
+  return hipSuccess;
+}
+
+}  // namespace
+
+// waves | splits << 8 for such a call
+extern "C" int ks_scaled_decode_shape(int num_seqs, int num_kv_heads, int max_blocks) {
+  const Shape s = decode_shape(num_seqs, num_kv_heads, max_blocks);
+  return s.waves | s.splits << 8;
+}
+
+// part_out and part_ml are read where the shape has several splits
+extern "C" hipError_t ks_paged_attention_decode_scaled(
+    void* out, const void* q, const void* k_cache, const void* v_cache,
+    const void* k_scale, const void* v_scale, const void* block_tables,
+    const void* context_lens, float scale, int num_seqs, int num_heads, int num_kv_heads,
+    int head_dim, int max_blocks, int pages, long q_row_stride, int shape,
+    void* part_out, void* part_ml, int window, hipStream_t stream) {
+  if (num_kv_heads < 1 || num_heads % num_kv_heads != 0 || pages < 1)
+    return hipErrorInvalidValue;
+  const int group = num_heads / num_kv_heads;
+  const int waves = shape & 255;
+  const int splits = part_out && part_ml ? shape >> 8 : 1;
+  if (group < 1 || group > 8 || splits < 1 || (waves != 4 && waves != 8))
+    return hipErrorInvalidValue;
+  if (num_seqs == 0) return hipSuccess;
+  const ScaledDecode p{out,
+                       (const short*)q,
+                       (const unsigned char*)k_cache,
+                       (const unsigned char*)v_cache,
+                       Scales{(const unsigned char*)k_scale, (const unsigned char*)v_scale,
+                              pages},
+                       (const int*)block_tables,
+                       (const int*)context_lens,
+                       score_scale(scale),
+                       num_heads,
+                       num_kv_heads,
+                       group,
+                       max_blocks,
+                       q_row_stride,
+                       splits,
+                       (float*)part_out,
+                       (float*)part_ml,
+                       window};
+  if (head_dim == 128) return launch_scaled<128>(p, num_seqs, waves, stream);
+  if (head_dim == 64) return launch_scaled<64>(p, num_seqs, waves, stream);
+  return hipErrorInvalidValue;
+}

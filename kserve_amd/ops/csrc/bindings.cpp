@@ -43,6 +43,7 @@ hipError_t ks_paged_attention_decode_scaled(void*, const void*, const void*, con
                                             const void*, float, int, int, int, int, int,
                                             int, long, int, void*, void*, int,
                                             hipStream_t);
+int ks_scaled_decode_shape(int, int, int);
 hipError_t ks_context_prefill_scaled(void*, const void*, const void*, const void*,
                                      const void*, const void*, const void*, const void*,
                                      const void*, int, int, int, int, int, int, int, float,
@@ -212,8 +213,10 @@ void check_scaled_pages(const at::Tensor& k_cache, const at::Tensor& v_cache,
   for (const at::Tensor* s : {&k_scale, &v_scale})
     TORCH_CHECK(s->scalar_type() == at::kFloat8_e8m0fnu && s->dim() == 2 &&
                     s->size(0) == k_cache.size(0) && s->size(1) == k_cache.size(1) &&
-                    s->is_contiguous() && s->device() == dev,
-                "scaled pages: scales float8_e8m0fnu [pages, kv_heads], dense");
+                    s->is_contiguous() && s->device() == dev &&
+                    (uintptr_t)s->data_ptr() % 4 == 0,
+                "scaled pages: scales float8_e8m0fnu [pages, kv_heads], dense and 4-byte "
+                "aligned");
 }
 
 void write_scaled_pages(at::Tensor& k, at::Tensor& v, at::Tensor& k_cache,
@@ -318,7 +321,8 @@ void paged_attention_decode_scaled(at::Tensor& out, at::Tensor& q, at::Tensor& k
   TORCH_CHECK(H / Hkv <= 8, "scaled pages: groups of up to 8 heads in decode");
   const c10::DeviceGuard guard(q.device());
   const int max_blocks = block_tables.size(1);
-  const int n_splits = ks_paged_decode_splits(S, Hkv, max_blocks, D, 1);
+  const int shape = ks_scaled_decode_shape(S, Hkv, max_blocks);
+  const int n_splits = shape >> 8;
   at::Tensor part_out, part_ml;
   void *po = nullptr, *pml = nullptr;
   if (n_splits > 1) {
@@ -332,7 +336,7 @@ void paged_attention_decode_scaled(at::Tensor& out, at::Tensor& q, at::Tensor& k
                 out.data_ptr(), q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(),
                 k_scale.data_ptr(), v_scale.data_ptr(), block_tables.data_ptr(),
                 context_lens.data_ptr(), (float)scale, S, H, Hkv, D, max_blocks,
-                (int)k_cache.size(0), (long)q.stride(0), n_splits, po, pml, (int)window,
+                (int)k_cache.size(0), (long)q.stride(0), shape, po, pml, (int)window,
                 current_stream()),
             "paged_attention_decode");
 }

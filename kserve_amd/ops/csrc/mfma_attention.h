@@ -28,7 +28,7 @@ enum Src {
   PAGES_DMA,  // bf16 pages of 16 tokens, 16-byte aligned: straight into LDS
   PAGES_REG,  // bf16 pages at any alignment: through registers
   PAGES_FP8,  // E4M3 pages, widened to bf16 on the way
-  PAGES_FP8S,  // the same under a power of two per page and KV head
+  PAGES_FP8S,  // the same under a power of two per page and KV head (prefill)
 };
 constexpr bool byte_pages(int src) { return src == PAGES_FP8 || src == PAGES_FP8S; }
 
@@ -121,8 +121,15 @@ __device__ __forceinline__ float half_sum(float x) {
 
 // 2^e as the widening conversions take it, from e's E8M0 byte (0, 2^-127, as the least
 // normal number: a page that holds nothing)
-__device__ __forceinline__ float page_scale(unsigned char e) {
-  return __uint_as_float(max((unsigned int)e, 1u) << 23);
+__device__ __forceinline__ float page_scale(unsigned int e) {
+  return __uint_as_float(max(e, 1u) << 23);
+}
+
+// byte `at` (the same for a wave) of bytes that begin at a multiple of four: by the
+// scalar unit, which loads whole words
+__device__ __forceinline__ unsigned int scalar_byte(const unsigned char* bytes, long at) {
+  const unsigned int word = reinterpret_cast<const unsigned int*>(bytes)[at >> 2];
+  return word >> ((unsigned int)at & 3) * 8 & 255;
 }
 
 // four E4M3 bytes each of two pages, times the pages' powers of two, as bf16 (exact: 4
@@ -334,7 +341,7 @@ __global__ __launch_bounds__(256, 2) void prefill_attention_kernel(
     return reinterpret_cast<const char*>(base) + at * ES;
   };
   uint2 raw8[byte_pages(SRC) ? 2 * NI : 1];
-  unsigned char exps[2];  // PAGES_FP8S: of the rows in raw8 (a wave's are one page's)
+  unsigned int exps[2];  // PAGES_FP8S: of the rows in raw8 (a wave's are one page's)
   short8_t raw16[!DMA && !byte_pages(SRC) ? 2 * NI : 1];
   // DMA: fills buffer `buf`; otherwise the rows wait in registers for commit()
   auto stage_rows = [&](const char* kb, const char* vb, auto k_at, auto v_at, int buf) {
@@ -363,8 +370,8 @@ __global__ __launch_bounds__(256, 2) void prefill_attention_kernel(
     const char* kb = base_of(p.k, krs, g0, page);
     const char* vb = base_of(p.v, vrs, g0, page);
     if constexpr (SRC == PAGES_FP8S) {
-      exps[0] = p.s8.k[(long)page * p.Hkv + kvh];
-      exps[1] = p.s8.v[(long)page * p.Hkv + kvh];
+      exps[0] = scalar_byte(p.s8.k, (long)page * p.Hkv + kvh);
+      exps[1] = scalar_byte(p.s8.v, (long)page * p.Hkv + kvh);
     }
     if (KEEP && (t + 1) * KT <= len)
       stage_rows(kb, vb, [&](int i) { return koff[i]; }, [&](int i) { return voff[i]; }, buf);
@@ -684,7 +691,7 @@ __device__ __forceinline__ uint4 load16_nt(const char* from) {
 // launches with four use all of them: bf16 pages a pair for each (the LDS of the other
 // two is taken in any case).
 constexpr int WAVES = 2;
-constexpr int deep_pairs(int src) { return byte_pages(src) ? 16 : 2 * WAVES; }
+constexpr int deep_pairs(int src) { return src == PAGES_FP8 ? 16 : 2 * WAVES; }
 
 struct DecodeArgs {
   void* out;                // [S, H, D]
@@ -703,24 +710,7 @@ struct DecodeArgs {
   long sk, sv;
   const int* cu_q;  // [S+1] first token of a sequence (null: sequence s's is s)
   Extra x;
-  Scales s8;  // PAGES_FP8S
 };
-
-// keys of sequence s; of block-scaled pages as many as its table row has at most
-template <int SRC>
-__device__ __forceinline__ int context_of(const DecodeArgs& p, int s) {
-  return SRC == PAGES_FP8S ? min(p.ctx_lens[s], p.max_blocks * PAGE) : p.ctx_lens[s];
-}
-
-// 16-byte chunk that chunk c of a staged row of E4M3 pages is XORed with. Block-scaled
-// ones: the rows of both pages that one transposing load brings lie apart too, and heads
-// of 64 have four chunks.
-template <int D, int SRC>
-__device__ __forceinline__ int byte_swz(int r) {
-  if constexpr (SRC == PAGES_FP8) return (r >> 1) & 7;
-  else if constexpr (D == 128) return ((r >> 1) & 7) ^ (r >> 4 & 1) << 2;
-  else return ((r >> 2) & 3) ^ (r >> 4 & 1) << 1;
-}
 
 // query token of sequence s, -1 if it has none in this batch
 __device__ __forceinline__ int token_of(const DecodeArgs& p, int s) {
@@ -749,23 +739,22 @@ __device__ __forceinline__ float final_factor(const DecodeArgs& p, long tok, int
 // E4M3 pages: four waves per SIMD at least, or the compiler keeps the output in
 // accumulation registers and copies it out and back for every rescale.
 template <int D, int NW, int SRC, bool WIDE, int PARTS = 1>  // WIDE: groups of 6 to 8
-__global__ __launch_bounds__(NW * 64, byte_pages(SRC) ? 4 : 1) void paged_attention_kernel(
+__global__ __launch_bounds__(NW * 64, SRC == PAGES_FP8 ? 4 : 1) void paged_attention_kernel(
     const DecodeArgs p) {
   constexpr int KC = D / 32;           // contraction chunks of K Q^T
   constexpr int DB = D / 16;           // 16-column blocks of the output
   constexpr int ROWS = 2 * PAGE;       // rows of a stage (a pair of pages)
-  constexpr bool BYTES = byte_pages(SRC);
-  constexpr int ES = BYTES ? 1 : 2;
+  constexpr int ES = SRC == PAGES_FP8 ? 1 : 2;
   constexpr int STAGE = ROWS * D * ES;  // shorts: K rows, then V rows
   static_assert(SRC != PAGES_FP8 || D == 128, "E4M3 rows are 8 chunks");
   // elements per lane and load, loads per stage and tensor
-  constexpr int EPL = BYTES ? 16 : 8;
+  constexpr int EPL = SRC == PAGES_FP8 ? 16 : 8;
   constexpr int LPR = D / EPL;  // lanes per row
   constexpr int RPI = 64 / LPR;
   constexpr int NI = ROWS / RPI;
 
   const int kvh = blockIdx.x, s = blockIdx.y, split = blockIdx.z;
-  const int ctx = context_of<SRC>(p, s);
+  const int ctx = p.ctx_lens[s];
   const Range rg = page_range(ctx, p.window, p.x.chunk, p.n_splits, min(NW, WAVES));
   const int tok = token_of(p, s);
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -820,8 +809,6 @@ __global__ __launch_bounds__(NW * 64, byte_pages(SRC) ? 4 : 1) void paged_attent
   // page ids of pair n (past the end: the last page again, as its rows are)
   auto pages_of = [&](int n) {
     const int a = min(rg.first + 2 * n, rg.last), b = min(a + 1, rg.last);
-    if constexpr (SRC == PAGES_FP8S)
-      return Pages{min(max(bt[a], 0), p.s8.pages - 1), min(max(bt[b], 0), p.s8.pages - 1)};
     return Pages{bt[a], bt[b]};
   };
   // where this lane's bytes of load i come from; rows past the context repeat
@@ -836,17 +823,8 @@ __global__ __launch_bounds__(NW * 64, byte_pages(SRC) ? 4 : 1) void paged_attent
            (row * (int)st + chunk * EPL) * ES;
   };
   uint4 raw[2 * NI];
-  unsigned char exps[4];  // of the pair in raw: K of both pages, V of both
   auto load = [&](int n) {
     const Pages pg = pages_of(n);
-    if constexpr (SRC == PAGES_FP8S) {
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        const long at = (long)(h ? pg.b : pg.a) * p.Hkv + kvh;
-        exps[h] = p.s8.k[at];
-        exps[2 + h] = p.s8.v[at];
-      }
-    }
 #pragma unroll
     for (int i = 0; i < NI; ++i) {
       raw[2 * i] = load16_nt(src(p.k_cache, p.sk, n, pg, i, lchunk));
@@ -860,7 +838,7 @@ __global__ __launch_bounds__(NW * 64, byte_pages(SRC) ? 4 : 1) void paged_attent
 #pragma unroll
       for (int kv = 0; kv < 2; ++kv) {
         char* row = reinterpret_cast<char*>(lds[wave]) + (kv * ROWS + r) * D * ES;
-        const int sw = BYTES ? byte_swz<D, SRC>(r) : kv ? v_swz<D>(r) : k_swz<D>(r);
+        const int sw = SRC == PAGES_FP8 ? (r >> 1) & 7 : kv ? v_swz<D>(r) : k_swz<D>(r);
         *reinterpret_cast<uint4*>(row + (lchunk ^ sw) * 16) = raw[2 * i + kv];
       }
     }
@@ -871,21 +849,30 @@ __global__ __launch_bounds__(NW * 64, byte_pages(SRC) ? 4 : 1) void paged_attent
   int kaddr[KC];
 #pragma unroll
   for (int c = 0; c < KC; ++c)
-    kaddr[c] = BYTES
-                   ? col * D + ((2 * c + (g >> 1)) ^ byte_swz<D, SRC>(col)) * 16 + (g & 1) * 8
+    kaddr[c] = SRC == PAGES_FP8
+                   ? col * D + ((2 * c + (g >> 1)) ^ (col >> 1)) * 16 + (g & 1) * 8
                    : (col * D + ((4 * c + g) ^ k_swz<D>(col)) * 8) * 2;
   // Transposing load: lane i of 16 brings key i/4, columns 4 (i%4) .. + 3 and
   // receives column i of its four keys; of E4M3 key i/2, columns 8 (i%2) .. + 7 and
   // column i of eight keys, the fragment's of both pages.
-  const int vrow = BYTES ? (col >> 3) * PAGE + g * 4 + ((col >> 1) & 3)
+  const int vrow = SRC == PAGES_FP8 ? (col >> 3) * PAGE + g * 4 + ((col >> 1) & 3)
                                     : g * 4 + (col >> 2);
   int vaddr[DB];
 #pragma unroll
   for (int b = 0; b < DB; ++b)
-    vaddr[b] = BYTES
-                   ? (ROWS + vrow) * D + (b ^ byte_swz<D, SRC>(vrow)) * 16 + (col & 1) * 8
+    vaddr[b] = SRC == PAGES_FP8
+                   ? (ROWS + vrow) * D + (b ^ ((vrow >> 1) & 7)) * 16 + (col & 1) * 8
                    : (ROWS * D + vrow * D + ((2 * b + ((col & 3) >> 1)) ^ v_swz<D>(vrow)) * 8 +
                       (col & 1) * 4) * 2;
+  auto widen = [](uint2 x) {  // eight E4M3 bytes, exactly
+    uint4 o;
+    o.x = __builtin_bit_cast(unsigned int, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(x.x, 1.0f, false));
+    o.y = __builtin_bit_cast(unsigned int, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(x.x, 1.0f, true));
+    o.z = __builtin_bit_cast(unsigned int, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(x.y, 1.0f, false));
+    o.w = __builtin_bit_cast(unsigned int, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(x.y, 1.0f, true));
+    return __builtin_bit_cast(bf16x8_t, o);
+  };
+
   float c2 = p.scale * LOG2E;
   const bool flip = c2 < 0.f;
   c2 = fabsf(c2);
@@ -895,9 +882,6 @@ __global__ __launch_bounds__(NW * 64, byte_pages(SRC) ? 4 : 1) void paged_attent
 #pragma unroll
   for (int b = 0; b < DB; ++b) o[b] = f32x4_t{0.f, 0.f, 0.f, 0.f};
 
-  float pow2[4];  // of the pair that is multiplied: K of both pages, V of both
-#pragma unroll
-  for (int i = 0; i < 4; ++i) pow2[i] = 1.f;
   auto compute = [&](int n, const char* st) {
     f32x4_t sc[2];
 #pragma unroll
@@ -906,11 +890,9 @@ __global__ __launch_bounds__(NW * 64, byte_pages(SRC) ? 4 : 1) void paged_attent
       f32x4_t rest = sc[h];  // the products with the query's lower parts
 #pragma unroll
       for (int c = 0; c < KC; ++c) {
-        // (block-scaled: the second page's chunks are swizzled by half a row more)
-        const int at = SRC == PAGES_FP8S ? c ^ (h * KC / 2) : c;
-        const char* from = st + h * PAGE * D * ES + kaddr[at];
+        const char* from = st + h * PAGE * D * ES + kaddr[c];
         bf16x8_t a;
-        if constexpr (BYTES) a = widen_fp8(*reinterpret_cast<const uint2*>(from), pow2[h]);
+        if constexpr (SRC == PAGES_FP8) a = widen(*reinterpret_cast<const uint2*>(from));
         else a = *reinterpret_cast<const bf16x8_t*>(from);
         if constexpr (PARTS == 3) {
           rest = mfma16x16x32(a, qf[PARTS - 1][c], rest);
@@ -947,7 +929,7 @@ __global__ __launch_bounds__(NW * 64, byte_pages(SRC) ? 4 : 1) void paged_attent
     }
     const float mc = m * c2;
     bf16x8_t pf, pl;
-    if constexpr (WIDE || BYTES) {
+    if constexpr (WIDE || SRC == PAGES_FP8) {
 #pragma unroll
       for (int h = 0; h < 2; ++h)
 #pragma unroll
@@ -989,12 +971,10 @@ __global__ __launch_bounds__(NW * 64, byte_pages(SRC) ? 4 : 1) void paged_attent
         bf16x8_t v;
       } a;
       const char* a0 = st + vaddr[b];
-      if constexpr (BYTES) {
+      if constexpr (SRC == PAGES_FP8) {
         typedef int i2_t __attribute__((ext_vector_type(2)));
         typedef __attribute__((address_space(3))) i2_t lds2_t;
-        a.v = widen_pages(
-            __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr8_b64_v2i32((lds2_t*)a0)),
-            pow2[2], pow2[3]);
+        a.v = widen(__builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr8_b64_v2i32((lds2_t*)a0)));
       } else {
         typedef __attribute__((address_space(3))) s16x4_t lds4_t;
         a.h[0] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4_t*)a0);
@@ -1011,10 +991,6 @@ __global__ __launch_bounds__(NW * 64, byte_pages(SRC) ? 4 : 1) void paged_attent
   // the next pair's loads are under way while this one is multiplied
   for (int n = n_lo; n < n_hi; n += nw) {
     commit();
-    if constexpr (SRC == PAGES_FP8S) {
-#pragma unroll
-      for (int i = 0; i < 4; ++i) pow2[i] = page_scale(exps[i]);
-    }
     if (n + nw < n_hi) load(n + nw);
     compute(n, reinterpret_cast<const char*>(lds[wave]));
   }
@@ -1075,7 +1051,7 @@ __global__ __launch_bounds__(NW * 64, byte_pages(SRC) ? 4 : 1) void paged_attent
 
 // Combine split-context partials: one wave per (seq, head); a lane owns D/64
 // columns across all splits. Sequences that one split covers are done.
-template <int D, int NW, int PARTS = 1, int SRC = PAGES_REG>
+template <int D, int NW, int PARTS = 1>
 __global__ __launch_bounds__(256) void paged_attention_reduce_kernel(
     const DecodeArgs p, long total) {
   constexpr int ACC = D / 64;
@@ -1083,7 +1059,7 @@ __global__ __launch_bounds__(256) void paged_attention_reduce_kernel(
   const int lane = threadIdx.x & 63;
   if (sh >= total) return;
   const int s = sh / p.H;
-  const Range rg = page_range(context_of<SRC>(p, s), p.window, p.x.chunk, p.n_splits, min(NW, WAVES));
+  const Range rg = page_range(p.ctx_lens[s], p.window, p.x.chunk, p.n_splits, min(NW, WAVES));
   const int tok = token_of(p, s);
   if (rg.splits == 1 || tok < 0) return;
   const float* ml = p.part_ml + sh * p.n_splits * 2;
@@ -1157,14 +1133,14 @@ constexpr long UNSPLIT_BLOCKS = 192, FULL_BLOCKS = 512;
 
 template <int D, int SRC, int PARTS = 1>
 hipError_t launch_decode(const DecodeArgs& p, int num_seqs, hipStream_t stream) {
-  const bool few = p.max_blocks <= (byte_pages(SRC) ? 8 : 4);
+  const bool few = p.max_blocks <= (SRC == PAGES_FP8 ? 8 : 4);
   const long blocks = (long)num_seqs * p.Hkv;
   if (p.n_splits == 1 && blocks >= UNSPLIT_BLOCKS && blocks < FULL_BLOCKS) {
     launch_decode_waves<D, SRC, PARTS, 2 * WAVES>(p, num_seqs, stream);
   } else if (few && p.n_splits == 1 && blocks >= ONE_WAVE_BLOCKS) {
     launch_decode_waves<D, SRC, PARTS, 1>(p, num_seqs, stream);
   } else {
-    if constexpr (byte_pages(SRC)) {
+    if constexpr (SRC == PAGES_FP8) {
       if (p.n_splits <= 2 && blocks < MOST_DEEP_BLOCKS)
         launch_decode_waves<D, SRC, PARTS, 2 * WAVES>(p, num_seqs, stream);
       else
@@ -1176,7 +1152,7 @@ hipError_t launch_decode(const DecodeArgs& p, int num_seqs, hipStream_t stream) 
   HIP_CHECK_KERNEL();
   if (p.n_splits > 1) {
     const long sh = (long)num_seqs * p.H;
-    hipLaunchKernelGGL((paged_attention_reduce_kernel<D, WAVES, PARTS, SRC == PAGES_FP8S ? PAGES_FP8S : PAGES_REG>),
+    hipLaunchKernelGGL((paged_attention_reduce_kernel<D, WAVES, PARTS>),
                        dim3((unsigned)((sh + 3) / 4)), dim3(256), 0, stream, p, sh);
     HIP_CHECK_KERNEL();
   }
