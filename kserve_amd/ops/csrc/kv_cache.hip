@@ -105,56 +105,80 @@ struct ScaledWrite {
   int T, Hkv;
   unsigned int limit;  // slots of the cache
   long sk, sv;
-  int vec;  // rows are 16-byte aligned
 };
 
 constexpr int ROWS = 16;          // of a page
 constexpr int LEAST_SCALE = 27;   // 2^-100: far from what fp32 flushes
 constexpr int NO_SCALE = 255;     // E8M0's not-a-number: a page that holds nothing
+constexpr int INF = 0x7f80;       // bf16
 
-__device__ __forceinline__ float pow2(int e) {  // 2^e, 0 below 2^-126; e < 128
-  return __uint_as_float(e < -126 ? 0u : (unsigned int)(e + 127) << 23);
-}
+// 2^(e - 127) as the scaling conversions take it
+__device__ __forceinline__ float pow2(int e) { return __uint_as_float((unsigned int)e << 23); }
 
-__device__ __forceinline__ unsigned int to_fp8(float a, float b, float c, float d) {
-  const int lo = __builtin_amdgcn_cvt_pk_fp8_f32(a, b, 0, false);
-  return (unsigned int)__builtin_amdgcn_cvt_pk_fp8_f32(c, d, lo, true);
-}
+typedef short short2_t __attribute__((ext_vector_type(2)));
+typedef unsigned short ushort2_t __attribute__((ext_vector_type(2)));
+typedef __bf16 bf16x2_t __attribute__((ext_vector_type(2)));
 
-// eight bf16 numbers times inv (the largest of the finite ones 448 at most)
-__device__ __forceinline__ uint2 encode8(short8_t x, float inv, bool special) {
-  float f[8];
-#pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const short b = special && (x[i] & 0x7fff) >= 0x7f80 ? (short)0 : x[i];
-    f[i] = bf16_bits_to_float(b) * inv;
-  }
-  unsigned int w[2] = {to_fp8(f[0], f[1], f[2], f[3]), to_fp8(f[4], f[5], f[6], f[7])};
-  if (special) {
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const unsigned int m = x[i] & 0x7fff;
-      const unsigned int code = (m > 0x7f80 ? 0x7fu : 0x7eu) | (x[i] < 0 ? 0x80u : 0u);
-      if (m >= 0x7f80) w[i >> 2] = (w[i >> 2] & ~(0xffu << (i & 3) * 8)) | code << (i & 3) * 8;
-    }
-  }
-  return uint2{w[0], w[1]};
-}
-
-// eight E4M3 numbers times ratio, at most 1
-__device__ __forceinline__ uint2 rescale8(uint2 x, float ratio) {
-  unsigned int w[2] = {x.x, x.y};
+// eight numbers over 2^(e - 127), rounded to nearest even
+__device__ __forceinline__ uint2 encode8(uint4 x, int e) {
+  const unsigned int w[4] = {x.x, x.y, x.z, x.w};
+  unsigned int o[2];
 #pragma unroll
   for (int d = 0; d < 2; ++d) {
-    const float2_t lo = __builtin_amdgcn_cvt_pk_f32_fp8((int)w[d], false);
-    const float2_t hi = __builtin_amdgcn_cvt_pk_f32_fp8((int)w[d], true);
-    w[d] = to_fp8(lo[0] * ratio, lo[1] * ratio, hi[0] * ratio, hi[1] * ratio);
+    short2_t two = short2_t{0, 0};
+    two = __builtin_amdgcn_cvt_scalef32_pk_fp8_bf16(
+        two, __builtin_bit_cast(bf16x2_t, w[2 * d]), pow2(e), false);
+    two = __builtin_amdgcn_cvt_scalef32_pk_fp8_bf16(
+        two, __builtin_bit_cast(bf16x2_t, w[2 * d + 1]), pow2(e), true);
+    o[d] = __builtin_bit_cast(unsigned int, two);
   }
-  return uint2{w[0], w[1]};
+  return uint2{o[0], o[1]};
+}
+
+// the bytes of what is no finite number put in: 448 (all ones but the last bit) or none
+__device__ __forceinline__ uint2 encode_special8(uint4 x, uint2 codes) {
+  const unsigned int w[4] = {x.x, x.y, x.z, x.w};
+  unsigned int o[2] = {codes.x, codes.y};
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const int b = (int)(w[i >> 1] >> (i & 1) * 16 & 0xffff), m = b & 0x7fff;
+    const int at = (i & 3) * 8;
+    const unsigned int code = (m > INF ? 0x7fu : 0x7eu) | (unsigned int)b >> 15 << 7;
+    if (m >= INF) o[i >> 2] = (o[i >> 2] & ~(0xffu << at)) | code << at;
+  }
+  return uint2{o[0], o[1]};
+}
+
+// eight E4M3 numbers times 2^(from - to), at most 1
+__device__ __forceinline__ uint2 rescale8(uint2 x, int from, int to) {
+  auto two = [&](unsigned int w, bool high) {
+    return __builtin_bit_cast(
+        unsigned int, high ? __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, pow2(from), true)
+                           : __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, pow2(from), false));
+  };
+  return encode8(uint4{two(x.x, false), two(x.x, true), two(x.y, false), two(x.y, true)}, to);
+}
+
+// zeros with the signs of eight E4M3 numbers; what is no number stays none
+__device__ __forceinline__ uint2 no_numbers8(uint2 x) {
+  auto four = [](unsigned int w) {
+    const unsigned int sign = w & 0x80808080u;
+    // a carry into the top bit where the lower seven are all ones
+    const unsigned int none = ((w & 0x7f7f7f7fu) + 0x01010101u & 0x80808080u) >> 7;
+    return sign | none * 0x7f;
+  };
+  return uint2{four(x.x), four(x.y)};
+}
+
+// bf16 magnitudes of eight numbers, the largest of two at a time
+__device__ __forceinline__ ushort2_t largest8(uint4 x) {
+  auto two = [](unsigned int w) { return __builtin_bit_cast(ushort2_t, w & 0x7fff7fffu); };
+  return __builtin_elementwise_max(__builtin_elementwise_max(two(x.x), two(x.y)),
+                                   __builtin_elementwise_max(two(x.z), two(x.w)));
 }
 
 // token_of: the call's token of each row of the page, -1 without
-template <int D>
+template <int D, bool VEC>
 __device__ __forceinline__ void write_scaled_page(const ScaledWrite& p, const int* token_of,
                                                   long page, int task) {
   constexpr int LPR = D / 8, RPI = 64 / LPR, NI = ROWS / RPI;
@@ -167,78 +191,109 @@ __device__ __forceinline__ void write_scaled_page(const ScaledWrite& p, const in
   const short* src = (is_v ? p.v : p.k) + head * D + col;
   const long stride = is_v ? p.sv : p.sk;
   const int old_raw = *scale;
-  short8_t x[NI];
+  uint4 x[NI];
   int token[NI];
 #pragma unroll
   for (int i = 0; i < NI; ++i) {
     token[i] = token_of[i * RPI + lrow];
-    x[i] = short8_t{0, 0, 0, 0, 0, 0, 0, 0};
+    x[i] = uint4{0, 0, 0, 0};
     if (token[i] >= 0) {
       const short* from = src + token[i] * stride;
-      if (p.vec) {
-        x[i] = *reinterpret_cast<const short8_t*>(from);
+      if constexpr (VEC) {
+        x[i] = *reinterpret_cast<const uint4*>(from);
       } else {
+        short8_t e;
 #pragma unroll
-        for (int e = 0; e < 8; ++e) x[i][e] = from[e];
+        for (int j = 0; j < 8; ++j) e[j] = from[j];
+        x[i] = __builtin_bit_cast(uint4, e);
       }
     }
   }
-  int top = 0;
-  bool special = false;
+  ushort2_t two = largest8(x[0]);
 #pragma unroll
-  for (int i = 0; i < NI; ++i)
+  for (int i = 1; i < NI; ++i) two = __builtin_elementwise_max(two, largest8(x[i]));
+  int top = max((int)two[0], (int)two[1]);
+  const bool special = __any(top >= INF);
+  if (special) {  // the largest of the finite ones
+    top = 0;
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      const int m = x[i][e] & 0x7fff;
-      special |= m >= 0x7f80;
-      top = max(top, m >= 0x7f80 ? 0 : m);
+    for (int i = 0; i < NI; ++i) {
+      const short8_t e = __builtin_bit_cast(short8_t, x[i]);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) top = max(top, (e[j] & 0x7fff) >= INF ? 0 : e[j] & 0x7fff);
     }
+  }
 #pragma unroll
   for (int off = 32; off > 0; off >>= 1) top = max(top, __shfl_xor(top, off, 64));
-  special = __any(special);
   // 448 = 1.75 * 2^8
   const int need = max((top >> 7) - 8 + ((top & 0x7f) > 0x60 ? 1 : 0), LEAST_SCALE);
   const bool begun = token_of[0] >= 0;
   const int old = old_raw == NO_SCALE ? 0 : old_raw;
   const int now = begun ? need : max(old, need);
-  const float inv = pow2(127 - now);
   const bool rescale = !begun && now != old_raw;
-  const float ratio = old_raw == NO_SCALE ? 0.f : pow2(old - now);
 #pragma unroll
   for (int i = 0; i < NI; ++i) {
     unsigned char* to = rows + i * RPI * D;
-    if (token[i] >= 0)
-      *reinterpret_cast<uint2*>(to) = encode8(x[i], inv, special);
-    else if (rescale)
-      *reinterpret_cast<uint2*>(to) = rescale8(*reinterpret_cast<const uint2*>(to), ratio);
+    if (token[i] >= 0) {
+      uint2 codes = encode8(x[i], now);
+      if (special) codes = encode_special8(x[i], codes);
+      *reinterpret_cast<uint2*>(to) = codes;
+    } else if (rescale) {
+      // from 2^-126 at least: what is smaller by 2^26 than the new scale is 0 in any case
+      uint2 codes = rescale8(*reinterpret_cast<const uint2*>(to), max(old, 1), now);
+      if (old_raw == NO_SCALE) codes = no_numbers8(*reinterpret_cast<const uint2*>(to));
+      *reinterpret_cast<uint2*>(to) = codes;
+    }
   }
   if (lane == 0 && now != old_raw) *scale = (unsigned char)now;
 }
 
-// `per` consecutive tokens to a block
-template <int D>
-__global__ __launch_bounds__(1024) void write_scaled_kernel(const ScaledWrite p, const int per) {
+// `per` (64 at most) consecutive tokens to a block; VEC: rows and the slot map are 16-byte
+// aligned
+template <int D, bool VEC>
+__global__ __launch_bounds__(512, 6) void write_scaled_kernel(const ScaledWrite p, const int per) {
   __shared__ int token_of[ROWS];
   __shared__ int taken;  // an earlier token's block writes this page
-  const int wave = threadIdx.x >> 6, waves = blockDim.x >> 6;
+  const int wave = threadIdx.x >> 6, waves = blockDim.x >> 6, lane = threadIdx.x & 63;
+  const int first = blockIdx.x * per;
   auto page_of = [&](int slot) { return (unsigned int)slot < p.limit ? slot >> 4 : -1; };
-  const int end = min((int)blockIdx.x * per + per, p.T);
-  for (int t = blockIdx.x * per; t < end; ++t) {
-    const int page = page_of(p.slots[t]);
-    if (page < 0 || (t > 0 && page_of(p.slots[t - 1]) == page)) continue;
+  // the first tokens of runs in one page: one to a lane
+  const int mine = min(first + lane, p.T - 1);
+  const int page_here = page_of(p.slots[mine]);
+  const int page_before = mine > 0 ? page_of(p.slots[mine - 1]) : -1;
+  unsigned long todo = __ballot(lane < per && first + lane < p.T && page_here >= 0 &&
+                                page_here != page_before);
+  while (todo) {
+    const int at = __builtin_ctzl(todo);
+    todo &= todo - 1;
+    const int t = first + at;
+    const int page = __builtin_amdgcn_readlane(page_here, at);
     if (threadIdx.x < ROWS) token_of[threadIdx.x] = -1;
     if (threadIdx.x == ROWS) taken = 0;
     __syncthreads();
-    for (int j = threadIdx.x; j < p.T; j += blockDim.x) {
+    auto here = [&](int slot) { return (unsigned int)slot >> 4 == (unsigned int)page; };
+    auto look = [&](int j) {
       const int slot = p.slots[j];
-      if (page_of(slot) != page) continue;
+      if (!here(slot)) return;
       if (j < t) taken = 1;
       else atomicMax(&token_of[slot & (ROWS - 1)], j);
+    };
+    // eight tokens at a time, looked at singly only where one of them is of this page
+    const int whole = VEC ? p.T & ~7 : 0;
+    for (int j = threadIdx.x * 8; j < whole; j += blockDim.x * 8) {
+      const int4 a = *reinterpret_cast<const int4*>(p.slots + j);
+      const int4 b = *reinterpret_cast<const int4*>(p.slots + j + 4);
+      if (here(a.x) | here(a.y) | here(a.z) | here(a.w) | here(b.x) | here(b.y) | here(b.z) |
+          here(b.w)) {
+#pragma unroll 1
+        for (int i = 0; i < 8; ++i) look(j + i);
+      }
     }
+    for (int j = whole + threadIdx.x; j < p.T; j += blockDim.x) look(j);
     __syncthreads();
     if (!taken)
-      for (int task = wave; task < 2 * p.Hkv; task += waves)
-        write_scaled_page<D>(p, token_of, page, task);
+      for (int task = blockIdx.y * waves + wave; task < 2 * p.Hkv; task += gridDim.y * waves)
+        write_scaled_page<D, VEC>(p, token_of, page, task);
     __syncthreads();
   }
 }
@@ -254,7 +309,8 @@ extern "C" hipError_t ks_write_scaled_pages(const void* k, const void* v, void* 
       (D != 64 && D != 128))
     return hipErrorInvalidValue;
   if (T == 0 || pages == 0) return hipSuccess;
-  const bool vec = ((((uintptr_t)k | (uintptr_t)v) & 15) | ((sk | sv) & 7)) == 0;
+  const bool vec =
+      ((((uintptr_t)k | (uintptr_t)v | (uintptr_t)slots) & 15) | ((sk | sv) & 7)) == 0;
   const ScaledWrite p{(const short*)k,
                       (const short*)v,
                       (unsigned char*)k_cache,
@@ -266,15 +322,22 @@ extern "C" hipError_t ks_write_scaled_pages(const void* k, const void* v, void* 
                       (int)Hkv,
                       (unsigned int)(pages < (1L << 27) ? pages * ROWS : 1L << 31),
                       sk,
-                      sv,
-                      vec};
-  const int per = T <= 1024 ? 1 : 4;
-  const dim3 grid((unsigned)((T + per - 1) / per));
-  const dim3 block(64 * (unsigned)(2 * Hkv < 16 ? 2 * Hkv : 16));
-  if (D == 128)
-    hipLaunchKernelGGL((write_scaled_kernel<128>), grid, block, 0, stream, p, per);
-  else
-    hipLaunchKernelGGL((write_scaled_kernel<64>), grid, block, 0, stream, p, per);
+                      sv};
+  const int per = T <= 1024 ? 1 : T >= 65536 ? 64 : (int)((T + 1023) / 1024);
+  // a page's heads, K and V, in blocks of up to eight waves
+  const long tasks = 2 * Hkv, parts = tasks <= 8 * 64 ? (tasks + 7) / 8 : 64;
+  const dim3 grid((unsigned)((T + per - 1) / per), (unsigned)parts);
+  const dim3 block(64 * (unsigned)(tasks < 8 ? tasks : 8));
+#define GO(DD, VV) \
+  hipLaunchKernelGGL((write_scaled_kernel<DD, VV>), grid, block, 0, stream, p, per)
+  if (D == 128) {
+    if (vec) GO(128, true);
+    else GO(128, false);
+  } else {
+    if (vec) GO(64, true);
+    else GO(64, false);
+  }
+#undef GO
   HIP_CHECK_KERNEL();
   return hipSuccess;
 }
