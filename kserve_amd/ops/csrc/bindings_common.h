@@ -215,13 +215,28 @@ std::vector<at::Tensor> paged_batch(at::Tensor& pages, at::Tensor& page_starts,
                   block_size >= 1 && block_size < (1L << 31) &&
                   (max_blocks == 0 || seqs <= ((1L << 31) - 1) / max_blocks),
               "build_paged_batch: sizes out of range");
-  const auto i32 = at::TensorOptions().dtype(at::kInt).device(dev);
-  std::vector<at::Tensor> out{at::empty({num_tokens}, i32.dtype(at::kLong)),
-                              at::empty({num_tokens}, i32),
-                              at::empty({seqs + 1}, i32),
-                              at::empty({seqs, max_blocks}, i32),
-                              at::empty({seqs}, i32),
-                              at::empty({num_tokens}, i32)};
+  // one allocation, each part where one of its own could be (six of them took 5 us of the
+  // host's 8)
+  int64_t bytes = 0;
+  auto room = [&](int64_t n) {
+    const int64_t at = bytes;
+    bytes += (n + 255) / 256 * 256;
+    return at;
+  };
+  const int64_t at[6] = {room(num_tokens * 8),     room(num_tokens * 4), room((seqs + 1) * 4),
+                         room(seqs * max_blocks * 4), room(seqs * 4),       room(num_tokens * 4)};
+  const at::Tensor all = at::empty({bytes}, at::TensorOptions().dtype(at::kByte).device(dev));
+  auto part = [&](int i, at::ScalarType type, c10::IntArrayRef sizes) {
+    at::Tensor t = at::detail::make_tensor<c10::TensorImpl>(
+        c10::Storage(all.storage()), all.key_set(), c10::scalarTypeToTypeMeta(type));
+    t.unsafeGetTensorImpl()->set_storage_offset(at[i] / c10::elementSize(type));
+    t.unsafeGetTensorImpl()->set_sizes_contiguous(sizes);
+    return t;
+  };
+  std::vector<at::Tensor> out{part(0, at::kLong, {num_tokens}), part(1, at::kInt, {num_tokens}),
+                              part(2, at::kInt, {seqs + 1}),
+                              part(3, at::kInt, {seqs, max_blocks}), part(4, at::kInt, {seqs}),
+                              part(5, at::kInt, {num_tokens})};
   check_hip(ks_paged_batch(pages.data_ptr(), page_starts.data_ptr(), computed.data_ptr(),
                            fresh.data_ptr(), pages.size(0), seqs, num_tokens, max_blocks,
                            block_size, out[0].data_ptr(), out[1].data_ptr(),

@@ -119,35 +119,45 @@ __device__ void token_part(const BatchArgs& p) {
 }
 
 __device__ void table_part(const BatchArgs& p) {
-  const long total = (long)p.S * p.width;
-  const long first = (long)(blockIdx.x - p.token_blocks) * TABLE;
+  const unsigned int total = (unsigned int)p.S * p.width;  // below 2^31
+  const unsigned int first = (blockIdx.x - p.token_blocks) * (unsigned int)TABLE;
   for (int step = 0; step < TABLE; step += 1024) {
-    const long at = first + step + threadIdx.x * 4;
+    const unsigned int at = first + step + threadIdx.x * 4;
     if (at >= total) break;
-    int s = (int)(at / p.width), c = (int)(at - (long)s * p.width);
-    int2 span{0, 0};
-    int held = -1;
-    int id[4];
+    int s = (int)(at / p.width), c = (int)(at - s * (unsigned int)p.width);
+    auto held_of = [&](int2 span) {
+      const long ctx = (long)max(p.computed[s], 0) + max(p.fresh[s], 0);
+      return (int)min((ctx + p.block - 1) / p.block, (long)span.y);
+    };
+    int2 span = page_span(p, s);
+    int held = held_of(span);
+    int4 id{0, 0, 0, 0};
+    if (c + 4 <= p.width) {  // of one row; at a multiple of 4 bytes only
+      if (c + 4 <= held) __builtin_memcpy(&id, p.pages + span.x + c, 16);
+      else if (c < held) {
+        id.x = p.pages[span.x + c];
+        if (c + 1 < held) id.y = p.pages[span.x + c + 1];
+        if (c + 2 < held) id.z = p.pages[span.x + c + 2];
+      }
+    } else {
+      int one[4] = {0, 0, 0, 0};
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      id[i] = 0;
-      if (at + i >= total) continue;
-      if (held < 0) {
-        span = page_span(p, s);
-        const long ctx = (long)max(p.computed[s], 0) + max(p.fresh[s], 0);
-        held = (int)min((ctx + p.block - 1) / p.block, (long)span.y);
+      for (int i = 0; i < 4; ++i) {
+        if (at + i >= total) continue;
+        if (c < held) one[i] = p.pages[span.x + c];
+        if (++c == p.width && ++s < p.S) {
+          c = 0;
+          span = page_span(p, s);
+          held = held_of(span);
+        }
       }
-      if (c < held) id[i] = p.pages[span.x + c];
-      if (++c == p.width) {
-        c = 0;
-        ++s;
-        held = -1;
-      }
+      id = int4{one[0], one[1], one[2], one[3]};
     }
     if (at + 4 <= total) {
-      *reinterpret_cast<int4*>(p.tables + at) = int4{id[0], id[1], id[2], id[3]};
+      *reinterpret_cast<int4*>(p.tables + at) = id;
     } else {
-      for (int i = 0; at + i < total; ++i) p.tables[at + i] = id[i];
+      const int one[4] = {id.x, id.y, id.z, id.w};
+      for (unsigned int i = 0; i < 3 && at + i < total; ++i) p.tables[at + i] = one[i];
     }
   }
 }
