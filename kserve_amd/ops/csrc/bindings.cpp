@@ -213,10 +213,8 @@ void check_scaled_pages(const at::Tensor& k_cache, const at::Tensor& v_cache,
   for (const at::Tensor* s : {&k_scale, &v_scale})
     TORCH_CHECK(s->scalar_type() == at::kFloat8_e8m0fnu && s->dim() == 2 &&
                     s->size(0) == k_cache.size(0) && s->size(1) == k_cache.size(1) &&
-                    s->is_contiguous() && s->device() == dev &&
-                    (uintptr_t)s->data_ptr() % 4 == 0,
-                "scaled pages: scales float8_e8m0fnu [pages, kv_heads], dense and 4-byte "
-                "aligned");
+                    s->is_contiguous() && s->device() == dev,
+                "scaled pages: scales float8_e8m0fnu [pages, kv_heads], dense");
 }
 
 void write_scaled_pages(at::Tensor& k, at::Tensor& v, at::Tensor& k_cache,
