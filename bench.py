@@ -704,9 +704,10 @@ def main():
     parser.add_argument("--multi-step", dest="multi_step", type=int, default=8,
                         help="decode iterations per hipGraph window")
     parser.add_argument("--kv-cache-dtype", type=str, default="auto",
-                        choices=["auto", "fp8"],
-                        help="opt-in fp8 E4M3 KV cache (NOT the headline "
-                             "config; bf16 compute is unchanged)")
+                        choices=["auto", "fp8", "fp8_scaled"],
+                        help="opt-in fp8 E4M3 KV cache, plain or block-scaled "
+                             "(NOT the headline config; bf16 compute is "
+                             "unchanged)")
     parser.add_argument("--hybrid-compare", type=str, default=None,
                         metavar="SIZE[,SIZE...]",
                         help="instead of the flagship workload: prefill and "

@@ -933,10 +933,21 @@ class CacheConfig:
     # "auto" stores KV in the model dtype (bf16). "fp8" stores OCP E4M3
     # bytes (scale 1.0): half the KV bandwidth/capacity; attention math
     # stays fp32/bf16 after in-register conversion. GQA group <= 4, D=128.
+    # "fp8_scaled" stores the same bytes under a power of two per page and KV head
+    # (ops.reshape_and_cache), so that no value saturates and small ones keep their
+    # bits. GQA group <= 8, D=64 or 128.
     kv_cache_dtype: str = "auto"
 
+    @property
+    def scaled(self) -> bool:
+        return self.kv_cache_dtype == "fp8_scaled"
+
+    def scale_bytes_per_block(self, kv_heads: int) -> int:
+        """Bytes of a layer's K and V scales of one page."""
+        return 2 * kv_heads if self.scaled else 0
+
     def cache_torch_dtype(self, model_dtype):
-        if self.kv_cache_dtype in ("fp8", "fp8_e4m3"):
+        if self.kv_cache_dtype in ("fp8", "fp8_e4m3", "fp8_scaled"):
             import torch
 
             return torch.float8_e4m3fn

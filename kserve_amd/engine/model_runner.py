@@ -41,7 +41,8 @@ class ModelRunner:
         self.model = model
         self.device = torch.device(device)
         self.is_cuda = self.device.type == "cuda"
-        self.kv_caches: List[Tuple[torch.Tensor, torch.Tensor]] = []
+        # K and V pages of each layer; block-scaled ones with K's and V's scales
+        self.kv_caches: List[Tuple[torch.Tensor, ...]] = []
         self.num_gpu_blocks = 0
         self.max_blocks_per_seq = (
             config.scheduler.max_model_len + config.cache.block_size - 1
@@ -70,7 +71,7 @@ class ModelRunner:
         self._pin_event = None
         self._bt_cache: Dict[str, object] = {}
         # host-DRAM KV offload tier (pinned) + dedicated copy stream
-        self.cpu_kv_caches: List[Tuple[torch.Tensor, torch.Tensor]] = []
+        self.cpu_kv_caches: List[Tuple[torch.Tensor, ...]] = []
         self.num_cpu_blocks = 0
         self._swap_stream = (
             torch.cuda.Stream() if self.is_cuda else None
@@ -110,6 +111,8 @@ class ModelRunner:
                     * self.config.cache.block_size
                     * self._num_local_layers()
                     // (tp * 2)
+                ) + self._num_local_layers() * self.config.cache.scale_bytes_per_block(
+                    max(1, m.num_kv_heads // tp)
                 )
             num_blocks = self.config.cache.num_gpu_blocks or max(
                 budget // per_block_bytes,
@@ -198,17 +201,26 @@ class ModelRunner:
             self.config.cache.block_size,
             m.head_dim,
         )
-        dtype = self.config.cache.cache_torch_dtype(self.model.dtype)
+        cache = self.config.cache
+        dtype = cache.cache_torch_dtype(self.model.dtype)
+        if cache.scaled and self.is_cuda and (
+            cache.block_size != 16 or m.head_dim not in (64, 128)
+            or m.num_heads > 8 * m.num_kv_heads
+        ):
+            raise ValueError(
+                "kv_cache_dtype fp8_scaled: pages of 16 tokens, heads of 64 or 128 and "
+                "up to 8 query heads to a KV head"
+            )
         # empty, not zeros: context_lens bound all reads, and zeroing a
         # 250 GB pool costs seconds of startup
         alloc = torch.empty if self.is_cuda else torch.zeros
-        self.kv_caches = [
-            (
-                alloc(shape, dtype=dtype, device=self.device),
-                alloc(shape, dtype=dtype, device=self.device),
-            )
-            for _ in range(self._num_local_layers())
-        ]
+
+        def pages():
+            return tuple(
+                alloc(shape, dtype=dtype, device=self.device) for _ in range(2)
+            ) + self._page_scales(num_blocks, kv_heads_local, device=self.device)
+
+        self.kv_caches = [pages() for _ in range(self._num_local_layers())]
         self.num_gpu_blocks = num_blocks
         self._allocate_cpu_kv()
         kv_gib = (
@@ -216,12 +228,27 @@ class ModelRunner:
             * m.head_dim * self._num_local_layers() * dtype.itemsize
         ) / (1 << 30)
         if dtype.itemsize == 1:
-            logger.info("KV cache dtype: fp8_e4m3 (scale 1.0)")
+            logger.info(
+                "KV cache dtype: fp8_e4m3 (%s)",
+                "a power of two per page and head" if cache.scaled else "scale 1.0",
+            )
         logger.info(
             "KV cache: %d blocks x %d tokens (%.1f GiB, layout [blocks, kv_heads, block, head_dim])",
             num_blocks,
             self.config.cache.block_size,
             kv_gib,
+        )
+
+    def _page_scales(self, blocks: int, kv_heads: int, **kw) -> Tuple[torch.Tensor, ...]:
+        """K's and V's scales of a layer's pages, where they have any. (A page's are
+        written with its first row; zero bytes stand for the least scale.)"""
+        if not self.config.cache.scaled:
+            return ()
+        return tuple(
+            torch.zeros((blocks, kv_heads), dtype=torch.uint8, **kw).view(
+                torch.float8_e8m0fnu
+            )
+            for _ in range(2)
         )
 
     def _allocate_cpu_kv(self):
@@ -235,7 +262,7 @@ class ModelRunner:
         per_block = (
             2 * kv_heads_local * cache.block_size * m.head_dim
             * self._num_local_layers() * kv_dtype.itemsize
-        )
+        ) + self._num_local_layers() * cache.scale_bytes_per_block(kv_heads_local)
         n = cache.num_cpu_blocks
         if not n and cache.cpu_offload_bytes:
             n = int(cache.cpu_offload_bytes // per_block)
@@ -247,6 +274,7 @@ class ModelRunner:
             (
                 torch.empty(shape, dtype=kv_dtype, pin_memory=pin),
                 torch.empty(shape, dtype=kv_dtype, pin_memory=pin),
+                *self._page_scales(n, kv_heads_local, pin_memory=pin),
             )
             for _ in range(self._num_local_layers())
         ]
@@ -263,15 +291,13 @@ class ModelRunner:
         if not pairs:
             return
         def do_copies():
-            for layer, (gk, gv) in enumerate(self.kv_caches):
-                ck, cv = self.cpu_kv_caches[layer]
-                for a, b in pairs:
-                    if to_gpu:  # (cpu, gpu)
-                        gk[b].copy_(ck[a], non_blocking=True)
-                        gv[b].copy_(cv[a], non_blocking=True)
-                    else:       # (gpu, cpu)
-                        ck[b].copy_(gk[a], non_blocking=True)
-                        cv[b].copy_(gv[a], non_blocking=True)
+            for on_gpu, on_cpu in zip(self.kv_caches, self.cpu_kv_caches):
+                for gpu, cpu in zip(on_gpu, on_cpu):
+                    for a, b in pairs:
+                        if to_gpu:  # (cpu, gpu)
+                            gpu[b].copy_(cpu[a], non_blocking=True)
+                        else:       # (gpu, cpu)
+                            cpu[b].copy_(gpu[a], non_blocking=True)
         if self.is_cuda:
             ev_before = torch.cuda.Event()
             ev_before.record(torch.cuda.current_stream())
@@ -298,73 +324,66 @@ class ModelRunner:
 
         total = sum(batch.num_scheduled_tokens)
         tokens = np.empty(total, dtype=np.int64)
-        positions = np.empty(total, dtype=np.int64)
-        slots = np.empty(total, dtype=np.int32)
-        cu = [0]
         max_seqlen = 0
         last_token_idx: List[int] = []
         off = 0
-        bs = self.config.cache.block_size
         for req, n in zip(batch.requests, batch.num_scheduled_tokens):
             start = req.num_computed_tokens
-            end = start + n
-            tokens[off : off + n] = req.all_token_ids[start:end]
-            positions[off : off + n] = np.arange(start, end, dtype=np.int64)
-            # vectorized slot mapping from the block table
-            bt = np.asarray(
-                block_manager.get_block_table(req), dtype=np.int32
-            )
-            pos_range = np.arange(start, end, dtype=np.int64)
-            slots[off : off + n] = bt[pos_range // bs] * bs + (
-                pos_range % bs
-            ).astype(np.int32)
+            tokens[off : off + n] = req.all_token_ids[start : start + n]
             off += n
-            cu.append(cu[-1] + n)
             max_seqlen = max(max_seqlen, n)
             # (nothing scheduled so far: a row all the same, the batch's last)
-            last_token_idx.append((cu[-1] or total) - 1)
+            last_token_idx.append((off or total) - 1)
         if logit_rows is None:
             sel = np.asarray(last_token_idx, dtype=np.int64)
         else:
             sel = torch.tensor(logit_rows, dtype=torch.int64, device="cpu").numpy()
-        arrays = [tokens, positions, sel, slots, np.asarray(cu, dtype=np.int32)]
+        arrays = [tokens, sel]
         if self._layout is not None:
-            counts = np.asarray(batch.num_scheduled_tokens, dtype=np.int64)
-            arrays.append(np.repeat(np.arange(len(counts), dtype=np.int32), counts))
             arrays.append(
                 np.asarray([r.state_slot for r in batch.requests], dtype=np.int32)
             )
         # chunked-prefill resume: any request with context already in pages
         # must attend to it — switch to the paged-context attention path
         # (models without an un-paged prefill kernel always take it)
-        if getattr(self.model, "paged_prefill_only", False) or (
+        paged = bool(getattr(self.model, "paged_prefill_only", False)) or (
             any(r.num_computed_tokens > 0 for r in batch.requests)
-            and self.kv_caches and self.kv_caches[0][0].numel() > 0
-        ):
-            nb_per = [
-                -(-(r.num_computed_tokens + n) // bs)
-                for r, n in zip(batch.requests, batch.num_scheduled_tokens)
-            ]
-            max_nb = max(nb_per)
-            btab = np.zeros((len(batch.requests), max_nb), dtype=np.int32)
-            ctx = np.empty(len(batch.requests), dtype=np.int32)
-            for i, (req, n) in enumerate(
-                zip(batch.requests, batch.num_scheduled_tokens)
-            ):
-                t = block_manager.get_block_table(req)
-                btab[i, : nb_per[i]] = t[: nb_per[i]]
-                ctx[i] = req.num_computed_tokens + n
-            arrays += [btab, ctx]
-        input_ids, pos, sel, slot_mapping, cu_seqlens, *rest = self._to_device(arrays)
+            and bool(self.kv_caches) and self.kv_caches[0][0].numel() > 0
+        )
+        (input_ids, sel, *slots), made = self._paged_batch(
+            batch.requests, batch.num_scheduled_tokens, block_manager, arrays, paged
+        )
         meta = AttentionMetadata(
-            is_prefill=True, slot_mapping=slot_mapping, cu_seqlens=cu_seqlens,
+            is_prefill=True, slot_mapping=made.slot_mapping, cu_seqlens=made.cu_seqlens,
             max_seqlen=max_seqlen,
         )
         if self._layout is not None:
-            meta.seq_of_token, meta.state_slots, *rest = rest
-        if rest:
-            meta.block_tables, meta.context_lens = rest
-        return input_ids, pos, meta, sel
+            meta.seq_of_token, meta.state_slots = made.seq_of_token, slots[0]
+        if paged:
+            meta.block_tables, meta.context_lens = made.block_tables, made.context_lens
+        return input_ids, made.positions, meta, sel
+
+    def _paged_batch(self, requests, widths, block_manager, arrays, tables: bool = True):
+        """(the arrays on the device, what attention is told of the batch): the next
+        ``widths`` tokens of each request. Page lists and lengths go up with the arrays;
+        positions, slots and page tables (empty ones unless asked for) are made there."""
+        import numpy as np
+
+        bs = self.config.cache.block_size
+        computed = [r.num_computed_tokens for r in requests]
+        used = [-(-(c + n) // bs) for c, n in zip(computed, widths)]
+        lists = [block_manager.get_block_table(r)[:n] for r, n in zip(requests, used)]
+        ints = [
+            np.asarray([p for x in lists for p in x], dtype=np.int32),
+            np.cumsum([0] + [len(x) for x in lists], dtype=np.int32),
+            np.asarray(computed, dtype=np.int32),
+            np.asarray(widths, dtype=np.int32),
+        ]
+        out = self._to_device(list(arrays) + ints)
+        made = ops.build_paged_batch(
+            *out[len(arrays) :], sum(widths), max(used, default=0) if tables else 0, bs
+        )
+        return out[: len(arrays)], made
 
     def _to_device(self, arrays) -> List[torch.Tensor]:
         """The arrays on the device. A GPU gets them in one copy out of pinned
@@ -576,47 +595,24 @@ class ModelRunner:
         import numpy as np
 
         widths = [1 + len(d) for d in drafts]
-        total = sum(widths)
-        bs = self.config.cache.block_size
-        tokens = np.empty(total, dtype=np.int64)
-        positions = np.empty(total, dtype=np.int64)
-        slots = np.empty(total, dtype=np.int32)
+        tokens = np.empty(sum(widths), dtype=np.int64)
         cu = [0]
-        nb_per = []
         for req, d, w in zip(batch.requests, drafts, widths):
-            pos0 = req.num_computed_tokens
-            nb_per.append(-(-(pos0 + w) // bs))
-        max_nb = max(nb_per)
-        btab = np.zeros((len(batch.requests), max_nb), dtype=np.int32)
-        ctx = np.empty(len(batch.requests), dtype=np.int32)
-        off = 0
-        for i, (req, d, w) in enumerate(zip(batch.requests, drafts, widths)):
-            pos0 = req.num_computed_tokens
-            tokens[off] = req.all_token_ids[pos0]
-            tokens[off + 1 : off + w] = d
-            pr = np.arange(pos0, pos0 + w, dtype=np.int64)
-            positions[off : off + w] = pr
-            t = block_manager.get_block_table(req)
-            bt = np.asarray(t, dtype=np.int32)
-            slots[off : off + w] = bt[pr // bs] * bs + (pr % bs).astype(np.int32)
-            btab[i, : nb_per[i]] = bt[: nb_per[i]]
-            ctx[i] = pos0 + w
-            off += w
-            cu.append(off)
-        dev = self.device
-        from kserve_amd.models.llama import AttentionMetadata
-
+            tokens[cu[-1]] = req.all_token_ids[req.num_computed_tokens]
+            tokens[cu[-1] + 1 : cu[-1] + w] = d
+            cu.append(cu[-1] + w)
+        (input_ids,), made = self._paged_batch(
+            batch.requests, widths, block_manager, [tokens]
+        )
         meta = AttentionMetadata(
             is_prefill=True,
-            slot_mapping=torch.from_numpy(slots).to(dev, non_blocking=True),
-            cu_seqlens=torch.tensor(cu, dtype=torch.int32, device=dev),
+            slot_mapping=made.slot_mapping,
+            cu_seqlens=made.cu_seqlens,
             max_seqlen=max(widths),
-            block_tables=torch.from_numpy(btab).to(dev, non_blocking=True),
-            context_lens=torch.from_numpy(ctx).to(dev, non_blocking=True),
+            block_tables=made.block_tables,
+            context_lens=made.context_lens,
         )
-        input_ids = torch.from_numpy(tokens).to(dev, non_blocking=True)
-        pos = torch.from_numpy(positions).to(dev, non_blocking=True)
-        hidden = self.model(input_ids, pos, self.kv_caches, meta)
+        hidden = self.model(input_ids, made.positions, self.kv_caches, meta)
         return self.model.compute_logits(hidden), cu
 
     # -- hipGraph capture ------------------------------------------------------

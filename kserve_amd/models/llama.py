@@ -86,13 +86,15 @@ class LlamaAttention(nn.Module):
         hidden: torch.Tensor,  # [T, H]
         positions: torch.Tensor,  # [T]
         cos_sin_cache: torch.Tensor,
-        kv_cache: Tuple[torch.Tensor, torch.Tensor],
+        kv_cache: Tuple[torch.Tensor, ...],
         meta: AttentionMetadata,
         add_norm=None,  # see RowParallelLinear.forward
     ):
         T = hidden.shape[0]
-        k_cache, v_cache = kv_cache
-        rotate = (positions, cos_sin_cache, k_cache, v_cache, meta.slot_mapping)
+        # (a block-scaled cache: also the scales of K's and V's pages)
+        k_cache, v_cache, *scales = kv_cache
+        scaled = dict(zip(("k_scale", "v_scale"), scales))
+        rotate = (positions, cos_sin_cache, k_cache, v_cache, meta.slot_mapping, *scales)
         # q, k, v: strided views into the fused qkv output; kernels take row
         # strides
         if meta.lora is None:
@@ -113,7 +115,7 @@ class LlamaAttention(nn.Module):
                 out = ops.context_attention_varlen(
                     q, k_cache, v_cache, meta.block_tables, meta.cu_seqlens,
                     meta.context_lens, meta.max_seqlen, self.scale,
-                    window=self.sliding_window,
+                    window=self.sliding_window, **scaled,
                 )
             else:
                 out = ops.flash_prefill_varlen(
@@ -123,7 +125,7 @@ class LlamaAttention(nn.Module):
         else:
             out = ops.paged_attention_decode(
                 q, k_cache, v_cache, meta.block_tables, meta.context_lens,
-                self.scale, window=self.sliding_window,
+                self.scale, window=self.sliding_window, **scaled,
             )
         o_in = out.reshape(T, -1)
         o_delta = (
@@ -450,7 +452,7 @@ class LlamaForCausalLM(nn.Module):
         self,
         input_ids: torch.Tensor,  # [T]
         positions: torch.Tensor,  # [T]
-        kv_caches: List[Tuple[torch.Tensor, torch.Tensor]],
+        kv_caches: List[Tuple[torch.Tensor, ...]],
         meta: AttentionMetadata,
     ) -> torch.Tensor:
         st = comm.get_state()

@@ -1021,10 +1021,18 @@ def _rope_cache_direct(positions, q, k, v, cos_sin, k_cache, v_cache, slots) -> 
 def rope_and_cache(
     positions: torch.Tensor, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
     cos_sin_cache: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
-    slot_mapping: torch.Tensor,
+    slot_mapping: torch.Tensor, k_scale: Optional[torch.Tensor] = None,
+    v_scale: Optional[torch.Tensor] = None,
 ) -> Tuple[torch.Tensor, torch.Tensor]:
     """Rotates q and k (in place on the GPU) and scatters k and v into their
-    pages (an empty k_cache: no scatter); returns q and k."""
+    pages (an empty k_cache: no scatter; block-scaled ones with ``k_scale`` and
+    ``v_scale``, see ``reshape_and_cache``); returns q and k."""
+    if k_scale is not None or v_scale is not None:
+        none = k_cache[:0]
+        q, k = rope_and_cache(positions, q, k, v, cos_sin_cache, none, none, slot_mapping)
+        if k_cache.numel() > 0:
+            reshape_and_cache(k, v, k_cache, v_cache, slot_mapping, k_scale, v_scale)
+        return q, k
     if q.is_cuda and _rope_cache_direct(
         positions, q, k, v, cos_sin_cache, k_cache, v_cache, slot_mapping
     ):
@@ -1043,10 +1051,21 @@ def linear_rope_and_cache(
     x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor],
     heads: int, kv_heads: int, positions: torch.Tensor,
     cos_sin_cache: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
-    slot_mapping: torch.Tensor,
+    slot_mapping: torch.Tensor, k_scale: Optional[torch.Tensor] = None,
+    v_scale: Optional[torch.Tensor] = None,
 ) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
     """q, k, v [T, heads, D] = x @ weight^T (+ bias) with ``rope_and_cache``
     applied. Few rows: its kernel adds the GEMM's splits."""
+    if k_scale is not None or v_scale is not None:
+        # (a page's scale is that of all its new rows, so they are written once whole)
+        none = k_cache[:0]
+        q, k, v = linear_rope_and_cache(
+            x, weight, bias, heads, kv_heads, positions, cos_sin_cache, none, none,
+            slot_mapping,
+        )
+        if k_cache.numel() > 0:
+            reshape_and_cache(k, v, k_cache, v_cache, slot_mapping, k_scale, v_scale)
+        return q, k, v
     T, D = x.shape[0], weight.shape[0] // (heads + 2 * kv_heads)
 
     def parts(qkv):

@@ -110,8 +110,8 @@ class QKVParallelLinear(nn.Module):
 
     def forward(self, x: torch.Tensor, rotate=None):
         """q, k, v as [T, heads * D]; with ``rotate`` (positions, cos_sin_cache,
-        k_cache, v_cache, slot_mapping) rotated, written to their pages and
-        shaped [T, heads, D]."""
+        k_cache, v_cache, slot_mapping and a block-scaled cache's scales) rotated,
+        written to their pages and shaped [T, heads, D]."""
         if rotate is not None:
             return ops.linear_rope_and_cache(
                 x, self.weight, self.bias, self.heads_local, self.kv_heads_local,

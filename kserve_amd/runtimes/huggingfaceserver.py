@@ -188,7 +188,9 @@ def main(argv=None):
     # host-DRAM KV offload tier (LLMInferenceService KVCacheOffloadingSpec)
     parser.add_argument("--kv-offload-bytes", dest="kv_offload_bytes", type=int, default=0)
     parser.add_argument("--kv-cache-dtype", dest="kv_cache_dtype", default="auto",
-                        choices=["auto", "fp8"])
+                        choices=["auto", "fp8", "fp8_scaled"],
+                        help="fp8: E4M3 pages as they are; fp8_scaled: under a "
+                             "power of two per page and KV head")
     # LoRA adapter serving (reference: --enable-lora --lora-modules name=path)
     parser.add_argument("--speculative-draft-model",
                         dest="speculative_draft_model", default=None,

@@ -1,0 +1,312 @@
+"""The block-scaled cache as it is used: batch tables, writes, chunk and decode attention
+one after the other, on streams and in captured graphs, and in the engine
+(``kv_cache_dtype="fp8_scaled"``)."""
+
+import math
+
+import pytest
+import torch
+
+from kserve_amd import ops
+from kserve_amd.engine.block_manager import BlockManager
+from kserve_amd.engine.config import CacheConfig, EngineConfig, ModelConfig, SchedulerConfig
+from kserve_amd.engine.engine import LLMEngine
+from kserve_amd.engine.request import Request
+from kserve_amd.engine.sampling_params import SamplingParams
+from kserve_amd.engine.scheduler import ScheduledBatch
+from tests.test_scaled_pages import (
+    E4M3, E8M0, PAGE, context, decode, devices, held, near,
+)
+
+
+def empty_cache(pages, kv, D, dev):
+    return dict(
+        kc=torch.zeros((pages, kv, PAGE, D), dtype=torch.uint8, device=dev).view(E4M3),
+        vc=torch.zeros((pages, kv, PAGE, D), dtype=torch.uint8, device=dev).view(E4M3),
+        ks=torch.zeros((pages, kv), dtype=torch.uint8, device=dev).view(E8M0),
+        vs=torch.zeros((pages, kv), dtype=torch.uint8, device=dev).view(E8M0),
+    )
+
+
+def vec(x, dev):
+    return torch.tensor(x, dtype=torch.int32, device=dev)
+
+
+class TestTogether:
+    @pytest.mark.parametrize("dev", devices())
+    @pytest.mark.parametrize("heads, kv, D, window", [(8, 2, 128, 0), (6, 1, 64, 0), (8, 2, 64, 24)])
+    def test_prompts_in_chunks_then_tokens(self, dev, heads, kv, D, window):
+        """Three requests: two chunks of each prompt, then tokens one by one. What the
+        cache holds is near the rows that went in, and every output is that of what the
+        cache holds."""
+        g = torch.Generator().manual_seed(1)
+        lists = [[7, 2, 9, 4], [1, 8, 3, 5], [6, 10, 11, 12]]
+        done = [0, 0, 0]
+        sent = [[], [], []]  # (k, v) rows of each request
+        c = dict(empty_cache(13, kv, D, dev), window=window, scale=D**-0.5)
+        steps = [[20, 5, 1], [17, 1, 30], [1, 1, 1], [1, 1, 1], [9, 1, 2]] + [[1, 1, 1]] * 3
+        for new in steps:
+            T = sum(new)
+            made = ops.build_paged_batch(
+                vec([p for x in lists for p in x], dev), vec([0, 4, 8, 12], dev),
+                vec(done, dev), vec(new, dev), T, 4, PAGE,
+            )
+            qkv = torch.randn((T, heads + 2 * kv, D), generator=g)
+            qkv = (qkv * torch.exp(torch.randn((T, 1, 1), generator=g))).to(torch.bfloat16)
+            x = qkv.to(dev)
+            k, v = x[:, heads : heads + kv], x[:, heads + kv :]
+            ops.reshape_and_cache(
+                k, v, c["kc"], c["vc"], made.slot_mapping, k_scale=c["ks"], v_scale=c["vs"]
+            )
+            at = 0
+            for i, n in enumerate(new):
+                rows = qkv[at : at + n].double()
+                sent[i] += list(zip(rows[:, heads : heads + kv], rows[:, heads + kv :]))
+                done[i] += n
+                at += n
+            d = dict(c, q=x[:, :heads].contiguous(), table=made.block_tables,
+                     ctx=made.context_lens, cu=made.cu_seqlens)
+            host = {n: t.cpu() if torch.is_tensor(t) and t.dtype not in (E4M3, E8M0) else t
+                    for n, t in d.items()}
+            near(context(d), host, True)
+            if max(new) == 1:
+                near(decode(d), host)
+        for cache, scale, part in ((c["kc"], c["ks"], 0), (c["vc"], c["vs"], 1)):
+            values = held(cache, scale)
+            step = torch.exp2(scale.view(torch.uint8).cpu().double() - 127)
+            for pages, rows in zip(lists, sent):
+                for j, row in enumerate(rows):
+                    p = pages[j // PAGE]
+                    # half a step of E4M3 at each rounding, which a page's growing scale
+                    # repeats only where numbers are below its normal ones: those are off by
+                    # half their step of 2^-9 scales, at each of the scales up to the last
+                    # (2^-9 half and its halves before, 2^-9 in all)
+                    off = 2.0**-4 * row[part].abs() + 2.0**-9 * step[p][:, None]
+                    assert bool(((values[p, :, j % PAGE] - row[part]).abs() <= off).all())
+
+    @pytest.mark.gpu
+    def test_captured_and_replayed(self):
+        """A decode step in a graph, replayed over changing inputs with eager work between,
+        leaves what the eager calls leave."""
+        kv, heads, D, S = 2, 8, 128, 5
+        g = torch.Generator(device="cuda").manual_seed(2)
+        table = (torch.randperm(40, device="cuda", generator=g)[: S * 8] + 1).view(S, 8).int()
+        one, two = (empty_cache(42, kv, D, "cuda") for _ in range(2))
+        qkv = torch.zeros((S, heads + 2 * kv, D), dtype=torch.bfloat16, device="cuda")
+        slots = torch.zeros(S, dtype=torch.int32, device="cuda")
+        ctx = torch.ones(S, dtype=torch.int32, device="cuda")
+
+        def step(c):
+            ops.reshape_and_cache(
+                qkv[:, heads : heads + kv], qkv[:, heads + kv :], c["kc"], c["vc"], slots,
+                k_scale=c["ks"], v_scale=c["vs"],
+            )
+            d = dict(c, q=qkv[:, :heads], table=table, ctx=ctx, scale=0.1, window=0)
+            cu = torch.arange(S + 1, dtype=torch.int32, device="cuda")
+            return decode(d), context(dict(d, cu=cu), 1)
+
+        step(one)
+        for t in one.values():
+            t.view(torch.uint8).zero_()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            got = step(one)
+        for pos in range(100):
+            qkv.copy_(torch.randn(qkv.shape, device="cuda", generator=g) * math.exp(pos % 7))
+            slots.copy_(table[:, pos // PAGE] * PAGE + pos % PAGE)
+            ctx.fill_(pos + 1)
+            graph.replay()
+            kept = [t.clone() for t in got]
+            want = step(two)
+            torch.cuda.synchronize()
+            for a, b in zip(kept, want):
+                assert torch.equal(a, b), pos
+            for n in one:
+                assert torch.equal(one[n].view(torch.uint8), two[n].view(torch.uint8)), (pos, n)
+
+    @pytest.mark.gpu
+    def test_batch_tables_in_a_graph(self):
+        lens = torch.tensor([3, 5], dtype=torch.int32, device="cuda")
+        done = torch.zeros(2, dtype=torch.int32, device="cuda")
+        pages, starts = vec([4, 6, 9, 2], "cuda"), vec([0, 2, 4], "cuda")
+        ops.build_paged_batch(pages, starts, done, lens, 10, 2, PAGE)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            got = ops.build_paged_batch(pages, starts, done, lens, 10, 2, PAGE)
+        for a, b, c in [(3, 5, 0), (1, 9, 14), (0, 2, 20), (5, 0, 16), (12, 12, 8)]:
+            lens.copy_(torch.tensor([a, b]))
+            done.fill_(c)
+            graph.replay()
+            want = ops.build_paged_batch(pages.cpu(), starts.cpu(), done.cpu(), lens.cpu(), 10, 2, PAGE)
+            for x, y in zip(got, want):
+                assert torch.equal(x.cpu(), y)
+
+    @pytest.mark.gpu
+    def test_another_stream(self):
+        """On a stream of the caller's, with its workspaces."""
+        from tests.test_scaled_pages import attention_case, on
+
+        c = attention_case([5000, 4000], [1, 1], 8, 1, 128, 300)
+        d = on(c, "cuda")
+        stream = torch.cuda.Stream()
+        stream.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(stream):
+            outs = [decode(d) for _ in range(3)] + [context(dict(d)) for _ in range(2)]
+        torch.cuda.current_stream().wait_stream(stream)
+        for o in outs[:3]:
+            near(o, c)
+        for o in outs[3:]:
+            near(o, c, True)
+
+    @pytest.mark.gpu
+    def test_far_pages(self):
+        """Pages whose bytes lie past 2^32, and tokens of a table's far end."""
+        kv, D, pages = 8, 128, 300000  # 4.9 GB
+        kc = torch.zeros((pages, kv, PAGE, D), dtype=torch.uint8, device="cuda")
+        c = dict(kc=kc.view(E4M3), vc=kc.view(E4M3))
+        s = torch.zeros((pages, kv), dtype=torch.uint8, device="cuda")
+        c.update(ks=s.view(E8M0), vs=s.view(E8M0))
+        ids = vec([299999, 299000, 270000, 299998], "cuda")
+        g = torch.Generator().manual_seed(3)
+        k = torch.randn((50, kv, D), generator=g).to(torch.bfloat16).cuda()
+        made = ops.build_paged_batch(ids, vec([0, 4], "cuda"), vec([0], "cuda"), vec([50], "cuda"), 50, 4, PAGE)
+        # K and V are one buffer: written by K's rows, then again by the same as V's
+        ops.reshape_and_cache(k, k, c["kc"], c["vc"], made.slot_mapping, k_scale=c["ks"], v_scale=c["vs"])
+        q = torch.randn((1, 32, D), generator=g).to(torch.bfloat16).cuda()
+        d = dict(c, q=q, table=made.block_tables, ctx=made.context_lens, window=0, scale=D**-0.5,
+                 cu=vec([0, 1], "cuda"))
+        small = ids.long()
+        host = dict(
+            d, kc=c["kc"].view(torch.uint8)[small].cpu().view(E4M3), ks=s[small].cpu().view(E8M0),
+            q=q.cpu(), ctx=made.context_lens.cpu(), cu=torch.tensor([0, 1]),
+            table=torch.tensor([[0, 1, 2, 3]], dtype=torch.int32),
+        )
+        host.update(vc=host["kc"], vs=host["ks"])
+        near(decode(d), host)
+        near(context(d), host, True)
+
+
+def engine(kv_dtype, dev="cpu", eager=True, **cache):
+    torch.manual_seed(0)
+    gpu = dev == "cuda"
+    return LLMEngine(EngineConfig(
+        model=ModelConfig(
+            vocab_size=512, hidden_size=256, intermediate_size=512, num_layers=2, num_heads=4,
+            num_kv_heads=2, head_dim=64, max_position_embeddings=512, model_name="tiny",
+        ),
+        cache=CacheConfig(**{**dict(
+            block_size=16 if gpu else 4, num_gpu_blocks=96, kv_cache_dtype=kv_dtype), **cache}),
+        scheduler=SchedulerConfig(max_num_seqs=8, max_num_batched_tokens=256, max_model_len=256),
+        device=dev, eos_token_id=-1, enforce_eager=eager,
+    ))
+
+
+PROMPTS = [[1, 2, 3, 4, 5], list(range(7, 60)), [9] * 17]
+
+
+def tokens(e, n=24):
+    out = e.generate(PROMPTS, SamplingParams(temperature=0.0, max_tokens=n))
+    return [o.output_token_ids for o in out.values()]
+
+
+class TestEngine:
+    @pytest.mark.parametrize("dev", devices())
+    def test_generates(self, dev):
+        e = engine("fp8_scaled", dev)
+        for k, v, ks, vs in e.runner.kv_caches:
+            assert k.dtype == v.dtype == E4M3 and ks.dtype == vs.dtype == E8M0
+            assert ks.shape == vs.shape == k.shape[:2]
+        got, plain = tokens(e), tokens(engine("auto", dev))
+        assert all(len(x) == 24 for x in got)
+        # a prompt's first token does not read the cache
+        assert [x[0] for x in got] == [x[0] for x in plain]
+
+    @pytest.mark.gpu
+    def test_graphs_are_eager(self):
+        """Captured decode steps, padded ones among them, give the eager steps' tokens."""
+        assert tokens(engine("fp8_scaled", "cuda", eager=False)) == tokens(engine("fp8_scaled", "cuda"))
+
+    @pytest.mark.timeout(60)
+    @pytest.mark.parametrize("dev", devices())
+    def test_prompts_in_chunks(self, dev):
+        """Prompts that come in chunks, which attend to the cache."""
+        e = engine("fp8_scaled", dev)
+        e.config.scheduler.enable_chunked_prefill = True
+        e.config.scheduler.max_num_batched_tokens = 24
+        assert all(len(x) == 2 for x in tokens(e, 2))
+
+    @pytest.mark.parametrize("dev", devices())
+    def test_pages_move_with_their_scales(self, dev):
+        e = engine("fp8_scaled", dev, num_cpu_blocks=4)
+        r = e.runner
+        g = torch.Generator().manual_seed(5)
+        for layer in r.kv_caches:
+            for t in layer:
+                raw = torch.randint(0, 120, t.shape, generator=g, dtype=torch.int32)
+                t.view(torch.uint8).copy_(raw.to(torch.uint8))
+        want = [[t.view(torch.uint8)[7].clone() for t in layer] for layer in r.kv_caches]
+        r.swap_blocks([(7, 2)], to_gpu=False)
+        r.swap_blocks([(2, 9)], to_gpu=True)
+        if dev == "cuda":
+            torch.cuda.synchronize()
+        for layer, w in zip(r.kv_caches, want):
+            assert len(layer) == 4
+            for t, x in zip(layer, w):
+                assert torch.equal(t.view(torch.uint8)[9], x)
+
+    @pytest.mark.gpu
+    def test_refused_models(self):
+        with pytest.raises(ValueError):
+            LLMEngine(EngineConfig(
+                model=ModelConfig(
+                    vocab_size=64, hidden_size=128, intermediate_size=128, num_layers=1, num_heads=4,
+                    num_kv_heads=2, head_dim=32, max_position_embeddings=64, model_name="tiny"),
+                cache=CacheConfig(block_size=16, num_gpu_blocks=16, kv_cache_dtype="fp8_scaled"),
+                scheduler=SchedulerConfig(max_num_seqs=2, max_num_batched_tokens=64, max_model_len=64),
+                device="cuda", eos_token_id=-1,
+            ))
+
+    def test_sizes(self):
+        c = CacheConfig(kv_cache_dtype="fp8_scaled")
+        assert c.scaled and c.cache_torch_dtype(torch.bfloat16) == E4M3
+        assert c.scale_bytes_per_block(8) == 16
+        assert CacheConfig().scale_bytes_per_block(8) == 0
+        assert not CacheConfig(kv_cache_dtype="fp8").scaled
+
+
+class TestRunnerTables:
+    @pytest.mark.parametrize("dev", devices())
+    def test_prefill_and_draft_batches(self, dev):
+        """Positions, slots and tables of fresh and resumed prompts are those of the
+        requests' page lists."""
+        e = engine("auto", dev)
+        r, bs = e.runner, e.config.cache.block_size
+        manager = BlockManager(96, bs)
+        reqs = []
+        for i, (n, c) in enumerate([(40, 0), (33, 16), (70, 61)]):
+            q = Request(request_id=str(i), prompt_token_ids=list(range(n)),
+                        sampling_params=SamplingParams(max_tokens=4))
+            manager.allocate(q, n)
+            q.num_computed_tokens = c
+            reqs.append(q)
+        new = [40, 17, 5]
+        batch = ScheduledBatch(is_prefill=True, requests=reqs, num_scheduled_tokens=new)
+        ids, pos, meta, sel = r.prepare_prefill(batch, manager)
+        want = [(q.num_computed_tokens + j, manager.get_block_table(q))
+                for q, n in zip(reqs, new) for j in range(n)]
+        assert pos.tolist() == [p for p, _ in want]
+        assert ids.tolist() == [p for p, _ in want]
+        assert meta.slot_mapping.tolist() == [t[p // bs] * bs + p % bs for p, t in want]
+        assert meta.cu_seqlens.tolist() == [0, 40, 57, 62]
+        assert sel.tolist() == [39, 56, 61]
+        assert meta.context_lens.tolist() == [40, 33, 66]
+        used = [-(-c // bs) for c in (40, 33, 66)]
+        assert meta.block_tables.tolist() == [
+            (manager.get_block_table(q)[:u] + [0] * max(used))[: max(used)] for q, u in zip(reqs, used)
+        ]
+        for q in reqs:
+            q.num_computed_tokens = 0
+        batch = ScheduledBatch(is_prefill=True, requests=reqs, num_scheduled_tokens=[3, 2, 1])
+        _, pos, meta, sel = r.prepare_prefill(batch, manager)
+        assert pos.tolist() == [0, 1, 2, 0, 1, 0] and sel.tolist() == [2, 4, 5]
+        assert meta.block_tables is None and meta.context_lens is None
