@@ -40,6 +40,16 @@
 // ops/torch_ref.flash_prefill_varlen and context_attention_varlen.
 #include "mfma_attention.h"
 
+// few queries over block-scaled pages (attention_scaled.hip)
+extern "C" {
+int ks_scaled_few_columns(int max_q_len, int group);
+int ks_scaled_few_splits(int num_seqs, int max_q_len, int Hq, int Hkv, int max_nb);
+hipError_t ks_scaled_few(void*, const void*, const void*, const void*, const void*,
+                         const void*, const void*, const void*, const void*, int, int, int,
+                         int, int, int, int, float, long, int, long, int, void*, void*,
+                         hipStream_t);
+}
+
 namespace {
 
 using namespace mfma_attn;
@@ -80,6 +90,16 @@ __global__ __launch_bounds__(256) void prefill_attention_merge_kernel(
 // query heads that a block takes
 int heads_per_block(int group) { return group % 4 == 0 ? 4 : group % 2 == 0 ? 2 : 1; }
 
+template <int D>
+hipError_t merge(const PrefillArgs& p, hipStream_t stream) {
+  constexpr int ROWS = 256 / (D / 4);  // of a block
+  hipLaunchKernelGGL(prefill_attention_merge_kernel<D>,
+                     dim3((unsigned)((p.rows + ROWS - 1) / ROWS)), dim3(256), 0, stream,
+                     (short*)p.out, p.part_out, p.part_ml, p.n_splits, p.rows);
+  HIP_CHECK_KERNEL();
+  return hipSuccess;
+}
+
 template <int D, int SRC>
 hipError_t launch(PrefillArgs p, int num_seqs, int max_q_len, bool causal,
                   hipStream_t stream) {
@@ -104,14 +124,7 @@ hipError_t launch(PrefillArgs p, int num_seqs, int max_q_len, bool causal,
   }
 #undef GO
   HIP_CHECK_KERNEL();
-  if (p.n_splits > 1) {
-    constexpr int ROWS = 256 / (D / 4);  // of a block
-    hipLaunchKernelGGL(prefill_attention_merge_kernel<D>,
-                       dim3((unsigned)((p.rows + ROWS - 1) / ROWS)), dim3(256), 0, stream, (short*)p.out, p.part_out, p.part_ml,
-                       p.n_splits, p.rows);
-    HIP_CHECK_KERNEL();
-  }
-  return hipSuccess;
+  return p.n_splits > 1 ? merge<D>(p, stream) : hipSuccess;
 }
 
 bool aligned16(const void* a, const void* b) {
@@ -151,6 +164,18 @@ extern "C" hipError_t ks_context_prefill_varlen(
   return launch<128, PAGES_REG>(p, num_seqs, max_q_len, true, stream);
 }
 
+// key parts of such a call over block-scaled pages
+extern "C" int ks_context_scaled_splits(int num_seqs, long rows, int max_q_len, int Hq,
+                                        int Hkv, int max_nb, int window) {
+  if (num_seqs < 1 || max_q_len < 1 || Hkv < 1 || Hq % Hkv != 0) return 1;
+  if (ks_scaled_few_columns(max_q_len, Hq / Hkv) > 0) {
+    if (window > 0 && max_nb > (window + max_q_len) / PAGE + 2)
+      max_nb = (window + max_q_len) / PAGE + 2;
+    return ks_scaled_few_splits(num_seqs, max_q_len, Hq, Hkv, max_nb);
+  }
+  return ks_context_prefill_splits(num_seqs, rows, max_q_len, Hq, Hkv, max_nb, window);
+}
+
 extern "C" hipError_t ks_context_prefill_scaled(
     void* out, const void* q, const void* k_cache, const void* v_cache,
     const void* k_scale, const void* v_scale, const void* block_tables,
@@ -166,6 +191,14 @@ extern "C" hipError_t ks_context_prefill_scaled(
                       (float*)part_out, (float*)part_ml,
                       Scales{(const unsigned char*)k_scale, (const unsigned char*)v_scale,
                              pages}};
+  if (ks_scaled_few_columns(max_q_len, Hq / Hkv) > 0) {
+    const hipError_t e = ks_scaled_few(out, q, k_cache, v_cache, k_scale, v_scale, block_tables,
+                                       ctx_lens, cu_seqlens_q, num_seqs, max_q_len, Hq, Hkv,
+                                       head_dim, max_nb, pages, scale, sq, window, rows,
+                                       n_splits, part_out, part_ml, stream);
+    if (e != hipSuccess || n_splits == 1 || num_seqs == 0) return e;
+    return head_dim == 128 ? merge<128>(p, stream) : merge<64>(p, stream);
+  }
   if (head_dim == 128)
     return launch<128, PAGES_FP8S>(p, num_seqs, max_q_len, true, stream);
   if (head_dim == 64)

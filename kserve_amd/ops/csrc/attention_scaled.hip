@@ -376,6 +376,276 @@ __global__ __launch_bounds__(256) void scaled_decode_reduce_kernel(const ScaledD
       float_to_bf16_bits(x * (all > 0.f ? 1.f / all : 0.f));
 }
 
+// Few queries per sequence behind their context (drafts under verification, short turns):
+// decode's kernel with (query, head of the group) pairs of a sequence in 16 NB columns, each
+// with a limit of its own; bytes are widened once for all of them. Block c Hkv + head takes
+// the pairs from 16 NB c on. Weights are rounded to bf16, as in
+// the chunk kernel (2^-9 of values that are summed and then rounded so themselves).
+struct FewArgs {
+  ScaledDecode d;      // out, q: [T, H, D]
+  const int* cu_q;     // [S + 1]
+  int tokens;          // T
+  float* part_out;     // [n_splits, T, H, D]
+  float* part_ml;      // [n_splits, T, H, 2]: exponent, sum of weights or NO_KEYS
+};
+
+template <int D, int NW, int NB>
+__global__ __launch_bounds__(NW * 64, NB == 1 ? 3 : 2) void scaled_few_kernel(const FewArgs f) {
+  constexpr int KC = D / 32, DB = D / 16, ROWS = 2 * PAGE, TILE = PAGE * D, NI = D / 64;
+  constexpr int LPR = D / 16;
+  constexpr int COLS = 16 * NB;
+  constexpr int MERGE = COLS * (D + 4) + 2 * COLS;  // floats: the columns' sums, m and l
+  constexpr int AREA = MERGE * 4 > 2 * TILE ? MERGE * 4 : 2 * TILE;
+  const ScaledDecode& p = f.d;
+
+  const int kvh = blockIdx.x % p.Hkv, first_col = blockIdx.x / p.Hkv * COLS;
+  const int s = blockIdx.y, split = blockIdx.z;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int lane = threadIdx.x & 63;
+  const int G = p.group;
+  const int q_start = min(max(f.cu_q[s], 0), f.tokens);
+  const int q_len = min(f.cu_q[s + 1], f.tokens) - q_start;
+  const int cols = min(q_len * G - first_col, COLS);  // of the block
+  if (cols <= 0) return;
+  const int ctx = context_of(p, s);
+  const int start = ctx - q_len;  // position of query 0
+  auto low = [&](int pos) { return pos > 0 ? low_of(pos, p.window, 0) : 0; };
+  // keys of the block's first and last query
+  const int pos_lo = start + first_col / G, pos_hi = start + (first_col + cols - 1) / G;
+  const int key_lo = low(pos_lo), low_hi = low(pos_hi);
+  const int end = min(ctx, pos_hi + 1);  // keys
+  const int first = key_lo / PAGE, last = (end - 1) / PAGE;
+  const int pairs = end > 0 ? (last - first) / 2 + 1 : 0;
+  const int splits = max(1, min(p.n_splits, (pairs + NW - 1) / NW));
+  const int per = (pairs + splits - 1) / splits;
+  const int n_lo = split * per + wave;
+  const int n_hi = min((split + 1) * per, pairs);
+  const long rows = (long)f.tokens * p.H;
+  auto row_of = [&](int c) {  // (token, head) of the block's column c
+    return (long)(q_start + (first_col + c) / G) * p.H + kvh * G + (first_col + c) % G;
+  };
+  if (split >= splits || pairs == 0) {
+    for (int c = threadIdx.x; c < cols; c += NW * 64) {
+      if (p.n_splits > 1) f.part_ml[(split * rows + row_of(c)) * 2 + 1] = NO_KEYS;
+      else
+        for (int d = 0; d < D; ++d) reinterpret_cast<short*>(p.out)[row_of(c) * D + d] = 0;
+    }
+    return;
+  }
+  const int nw = min(max(n_hi - split * per, 1), NW);
+  if (wave >= nw) return;
+  const int col = lane & 15, g = lane >> 4;
+
+  __shared__ __attribute__((aligned(16))) char lds[NW][AREA];
+
+  const int* bt = p.block_tables + (long)s * p.max_blocks;
+  int id = 0;
+  unsigned int ks = 0, vs = 0;
+  auto fetch = [&](int n) {
+    id = bt[min(first + 2 * (n + (lane >> 1) * NW) + (lane & 1), last)];
+    id = min(max(id, 0), p.s8.pages - 1);
+    const long at = (long)id * p.Hkv + kvh;
+    ks = p.s8.k[at];
+    vs = p.s8.v[at];
+  };
+  uint4 kr[2][NI], vr[2][NI];
+  const unsigned int klane = col * D + g * 16, vlane = lane * 16;
+  auto tile = [&](const unsigned char* cache, int i, int h) {
+    const int page = __builtin_amdgcn_readlane(id, (i % BATCH) * 2 + h);
+    const char* at = reinterpret_cast<const char*>(cache) + ((long)page * p.Hkv + kvh) * TILE;
+    asm("" : "+s"(at));
+    return at;
+  };
+  auto load_k = [&](int i) {
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const char* from = tile(p.k_cache, i, h);
+#pragma unroll
+      for (int j = 0; j < NI; ++j)
+        kr[h][j] = *reinterpret_cast<const uint4*>(from + klane + j * 64);
+    }
+  };
+  auto load_v = [&](int i) {
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const char* from = tile(p.v_cache, i, h);
+#pragma unroll
+      for (int j = 0; j < NI; ++j)
+        vr[h][j] = *reinterpret_cast<const uint4*>(from + vlane + j * 1024);
+    }
+  };
+  if (n_lo < n_hi) {
+    fetch(n_lo);
+    load_k(0);
+    load_v(0);
+  }
+
+  bf16x8_t qf[NB][KC];
+  int my_pos[NB];
+  float c2 = p.scale * LOG2E;
+  {
+    const short flip = c2 < 0.f ? (short)0x8000 : (short)0;
+#pragma unroll
+    for (int b = 0; b < NB; ++b) {
+      const int c = first_col + min(b * 16 + col, cols - 1);
+      my_pos[b] = start + c / G;
+      const short* qp =
+          p.q + (long)(q_start + c / G) * p.sq + (long)(kvh * G + c % G) * D + g * 16;
+#pragma unroll
+      for (int k = 0; k < KC; ++k) {
+        short8_t x = *reinterpret_cast<const short8_t*>(qp + (k >> 1) * 64 + (k & 1) * 8);
+        x ^= flip;
+        qf[b][k] = __builtin_bit_cast(bf16x8_t, x);
+      }
+    }
+  }
+  c2 = fabsf(c2);
+
+  const int vrow = (col >> 3) * PAGE + g * 4 + ((col >> 1) & 3);
+  unsigned int vaddr = vrow * D + byte_swz<D>(vrow) * 16 + (col & 1) * 8;
+  unsigned int to[2];
+  to[0] = lane / LPR * D + ((lane % LPR) ^ byte_swz<D>(lane / LPR)) * 16;
+  to[1] = to[0] ^ (D / 2);
+
+  constexpr float ROOM = 8.f;
+  float mc[NB], l[NB];
+  f32x4_t o[NB][DB];
+#pragma unroll
+  for (int b = 0; b < NB; ++b) {
+    mc[b] = fmaxf(NO_MAX * c2, -3e38f);
+    l[b] = 0.f;
+#pragma unroll
+    for (int d = 0; d < DB; ++d) o[b][d] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+  }
+
+  for (int n = n_lo, i = 0; n < n_hi; n += NW, ++i) {
+    float k2[2], v2[2];
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      k2[h] = page_scale(__builtin_amdgcn_readlane(ks, (i % BATCH) * 2 + h));
+      v2[h] = page_scale(__builtin_amdgcn_readlane(vs, (i % BATCH) * 2 + h));
+    }
+    const bool more = n + NW < n_hi;
+    if (more && (i + 1) % BATCH == 0) fetch(n + NW);
+
+    f32x4_t sc[NB][2];
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+#pragma unroll
+      for (int b = 0; b < NB; ++b) sc[b][h] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int c = 0; c < KC; ++c) {
+        const uint4 x = kr[h][c >> 1];
+        const uint2 half = c & 1 ? uint2{x.z, x.w} : uint2{x.x, x.y};
+        const bf16x8_t a = widen_fp8(half, k2[h]);
+#pragma unroll
+        for (int b = 0; b < NB; ++b) sc[b][h] = mfma16x16x32(a, qf[b][c], sc[b][h]);
+      }
+    }
+    if (more) load_k(i + 1);
+    const int key0 = (first + 2 * n) * PAGE;
+    if (key0 + ROWS - 1 > pos_lo || key0 < low_hi) {
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          const int key = key0 + h * PAGE + g * 4 + r;
+#pragma unroll
+          for (int b = 0; b < NB; ++b)
+            sc[b][h][r] = key < ctx && key <= my_pos[b] && key >= low(my_pos[b]) ? sc[b][h][r]
+                                                                              : MASKED;
+        }
+#pragma unroll
+        for (int j = 0; j < NI; ++j) {
+          const int key = key0 + h * PAGE + j * (64 / LPR) + lane / LPR;
+          if (key >= ctx || key < key_lo) vr[h][j] = uint4{0, 0, 0, 0};
+        }
+      }
+    }
+    char* mine = lds[wave];
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+#pragma unroll
+      for (int j = 0; j < NI; ++j)
+        *reinterpret_cast<uint4*>(mine + to[(h + j) & 1] + (h * PAGE + j * (64 / LPR)) * D) =
+            vr[h][j];
+    if (more) load_v(i + 1);
+
+    bf16x8_t pf[NB];
+#pragma unroll
+    for (int b = 0; b < NB; ++b) {
+      float mx = fmaxf(fmaxf(fmaxf(sc[b][0][0], sc[b][0][1]), fmaxf(sc[b][0][2], sc[b][0][3])),
+                       fmaxf(fmaxf(sc[b][1][0], sc[b][1][1]), fmaxf(sc[b][1][2], sc[b][1][3])));
+      mx = column_max(mx) * c2;
+      if (__any(mx > mc[b] + ROOM)) {
+        const float mn = fmaxf(mc[b], mx);
+        const float r = __builtin_amdgcn_exp2f(mc[b] - mn);
+        mc[b] = mn;
+        l[b] *= r;
+#pragma unroll
+        for (int d = 0; d < DB; ++d) o[b][d] *= r;
+      }
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          const float w = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[b][h][r], c2, -mc[b]));
+          l[b] += w;
+          pf[b][h * 4 + r] = (__bf16)w;
+        }
+    }
+    asm("" : "+v"(vaddr));
+#pragma unroll
+    for (int d = 0; d < DB; ++d) {
+      typedef int i2_t __attribute__((ext_vector_type(2)));
+      typedef __attribute__((address_space(3))) i2_t lds2_t;
+      const char* a0 = mine + (vaddr ^ d * 16);
+      const bf16x8_t a = widen_pages(
+          __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr8_b64_v2i32((lds2_t*)a0)),
+          v2[0], v2[1]);
+#pragma unroll
+      for (int b = 0; b < NB; ++b) o[b][d] = mfma16x16x32(a, pf[b], o[b][d]);
+    }
+  }
+
+  float* mo = reinterpret_cast<float*>(lds[wave]);  // [COLS][D + 4], then m and l
+  float* mm = mo + COLS * (D + 4);
+#pragma unroll
+  for (int b = 0; b < NB; ++b) {
+    const float sum = column_sum(l[b]);
+#pragma unroll
+    for (int d = 0; d < DB; ++d)
+      *reinterpret_cast<f32x4_t*>(mo + (b * 16 + col) * (D + 4) + d * 16 + g * 4) = o[b][d];
+    if (lane < 16) {
+      mm[b * 16 + col] = mc[b];
+      mm[COLS + b * 16 + col] = sum;
+    }
+  }
+  __syncthreads();
+  constexpr int WF = AREA / 4;
+  const float* all = reinterpret_cast<const float*>(lds);
+  for (int i = threadIdx.x; i < cols * (D / 4); i += nw * 64) {
+    const int c = i / (D / 4), d = i % (D / 4) * 4;
+    float top = all[COLS * (D + 4) + c];
+    for (int w = 1; w < nw; ++w) top = fmaxf(top, all[w * WF + COLS * (D + 4) + c]);
+    float sum = 0.f;
+    f32x4_t acc = f32x4_t{0.f, 0.f, 0.f, 0.f};
+    for (int w = 0; w < nw; ++w) {
+      const float* a = all + w * WF;
+      const float r = __builtin_amdgcn_exp2f(a[COLS * (D + 4) + c] - top);
+      sum += r * a[COLS * (D + 4) + COLS + c];
+      acc += r * *reinterpret_cast<const f32x4_t*>(a + c * (D + 4) + d);
+    }
+    if (p.n_splits == 1) {
+      store4(p.out, row_of(c) * D + d, acc * (sum > 0.f ? 1.f / sum : 0.f), 0);
+    } else {
+      const long at = split * rows + row_of(c);
+      *reinterpret_cast<f32x4_t*>(f.part_out + at * D + d) = acc;
+      if (d == 0) *reinterpret_cast<float2_t*>(f.part_ml + at * 2) = float2_t{top, sum};
+    }
+  }
+}
+
 // Waves that share a context, 4 or 8, and its splits.
 //
 // From UNIT_BLOCKS blocks on, one to a compute unit, four waves and no splits (us, 4 x 1 / 8
@@ -467,4 +737,77 @@ extern "C" hipError_t ks_paged_attention_decode_scaled(
   if (head_dim == 128) return launch_scaled<128>(p, num_seqs, waves, stream);
   if (head_dim == 64) return launch_scaled<64>(p, num_seqs, waves, stream);
   return hipErrorInvalidValue;
+}
+
+// (query, head of a group) pairs of a sequence that the kernel for few queries takes, 32 to a
+// block. A chunk kernel's wave takes 32 queries of one head whatever there are, four such
+// waves a group's (32 / 8 heads of 128, us, chunk / few: 96 sequences of 2 queries after 1500
+// 110 / 53, of 5 115 / 66, of up to 10 116 / 94; 32 of 5 after 400 18.8 / 12.3; 4 of 5 after
+// 12900 53 / 33, of up to 10 54 / 46). At 64 pairs they are level (96 of 16 after 1500 120 /
+// 118, 4 of 16 after 12900 61 / 66), and beyond the chunk kernel is ahead (4 of 32 74 / 99).
+constexpr int FEW_COLUMNS = 64;
+
+// Column blocks of a launch over few queries (0: the chunk kernel's)
+extern "C" int ks_scaled_few_columns(int max_q_len, int group) {
+  const long cols = (long)max_q_len * group;
+  return cols < 1 ? 0 : cols <= 16 ? 1 : cols <= FEW_COLUMNS ? 2 : 0;
+}
+
+// part_out [splits, T, H, D] and part_ml [splits, T, H, 2]: left to be merged
+extern "C" hipError_t ks_scaled_few(
+    void* out, const void* q, const void* k_cache, const void* v_cache,
+    const void* k_scale, const void* v_scale, const void* block_tables,
+    const void* ctx_lens, const void* cu_q, int num_seqs, int max_q_len, int Hq, int Hkv,
+    int head_dim, int max_nb, int pages, float scale, long sq, int window, long rows,
+    int n_splits, void* part_out, void* part_ml, hipStream_t stream) {
+  const ScaledDecode d{out,
+                       (const short*)q,
+                       (const unsigned char*)k_cache,
+                       (const unsigned char*)v_cache,
+                       Scales{(const unsigned char*)k_scale, (const unsigned char*)v_scale,
+                              pages},
+                       (const int*)block_tables,
+                       (const int*)ctx_lens,
+                       score_scale(scale),
+                       Hq,
+                       Hkv,
+                       Hq / Hkv,
+                       max_nb,
+                       sq,
+                       n_splits,
+                       nullptr,
+                       nullptr,
+                       window};
+  const FewArgs f{d, (const int*)cu_q, (int)(rows / Hq), (float*)part_out, (float*)part_ml};
+  const int nb = ks_scaled_few_columns(max_q_len, Hq / Hkv);
+  if (nb == 0) return hipErrorInvalidValue;
+  if (num_seqs == 0) return hipSuccess;
+  const int groups = (max_q_len * (Hq / Hkv) + 16 * nb - 1) / (16 * nb);
+  const dim3 grid(Hkv * groups, num_seqs, n_splits);
+#define GO(DD, BB) \
+  hipLaunchKernelGGL((scaled_few_kernel<DD, 4, BB>), grid, dim3(256), 0, stream, f)
+  if (head_dim == 128) {
+    if (nb == 1) GO(128, 1);
+    else GO(128, 2);
+  } else if (head_dim == 64) {
+    if (nb == 1) GO(64, 1);
+    else GO(64, 2);
+  } else {
+    return hipErrorInvalidValue;
+  }
+#undef GO
+  HIP_CHECK_KERNEL();
+  return hipSuccess;
+}
+
+// key parts of such a launch
+extern "C" int ks_scaled_few_splits(int num_seqs, int max_q_len, int Hq, int Hkv, int max_nb) {
+  const int groups = (int)(((long)max_q_len * (Hq / Hkv) + 31) / 32);
+  const long blocks = (long)num_seqs * Hkv * groups, pairs = (max_nb + 1) / 2;
+  // (as for decode: a launch that merges costs what eight pairs of a wave take)
+  if (blocks <= 0 || blocks >= UNIT_BLOCKS || pairs <= 8 * SHORT) return 1;
+  long splits = (UNIT_BLOCKS + blocks / 2) / blocks;
+  const long most = (pairs + 7) / 8;  // two pairs for every wave
+  if (splits > most) splits = most;
+  return splits < 1 ? 1 : (int)splits;
 }

@@ -44,6 +44,7 @@ hipError_t ks_paged_attention_decode_scaled(void*, const void*, const void*, con
                                             int, long, int, void*, void*, int,
                                             hipStream_t);
 int ks_scaled_decode_shape(int, int, int);
+int ks_context_scaled_splits(int, long, int, int, int, int, int);
 hipError_t ks_context_prefill_scaled(void*, const void*, const void*, const void*,
                                      const void*, const void*, const void*, const void*,
                                      const void*, int, int, int, int, int, int, int, float,
@@ -425,8 +426,8 @@ void context_prefill_scaled(at::Tensor& out, at::Tensor& q, at::Tensor& k_cache,
   const int longest = (int)std::min<int64_t>(std::max<int64_t>(max_q_len, 0), q.size(0));
   const long rows = (long)q.size(0) * Hq;
   const int n_splits =
-      ks_context_prefill_splits((int)seqs, rows, longest, Hq, Hkv,
-                                (int)block_tables.size(1), (int)window);
+      ks_context_scaled_splits((int)seqs, rows, longest, Hq, Hkv, (int)block_tables.size(1),
+                               (int)window);
   TORCH_CHECK(seqs * n_splits < 65536, "scaled pages: sizes out of range");
   at::Tensor part_out, part_ml;
   void *po = nullptr, *pml = nullptr;

@@ -386,6 +386,34 @@ class TestContext:
         c = attention_case([3000, 2500], [20, 9], 8, 2, D, 120)
         near(context(on(c, "cuda")), c, True)
 
+    @pytest.mark.parametrize("dev", devices())
+    @pytest.mark.parametrize("D", [64, 128])
+    @pytest.mark.parametrize("window", [0, 1, 20])
+    @pytest.mark.parametrize(
+        "heads, kv, new",
+        [(1, 1, [1, 16, 3, 0]), (1, 1, [32, 1, 5, 17]), (8, 2, [8, 2, 5, 1]), (8, 2, [4, 0, 1, 3]),
+         (5, 1, [6, 6, 2, 1]), (16, 2, [4, 1, 3, 2]), (7, 1, [2, 4, 1, 3]), (22, 2, [2, 1, 2, 1]),
+         (1, 1, [40, 16, 64, 33]), (8, 2, [10, 16, 9, 2]), (7, 1, [8, 9, 5, 1])],
+    )
+    def test_few_queries(self, dev, D, window, heads, kv, new):
+        """As many as go beside one another in the columns of one product, of two, and of
+        two blocks."""
+        c = attention_case([40, 16, 177, 33], new, heads, kv, D, 150, window)
+        near(context(on(c, dev)), c, True)
+
+    @pytest.mark.gpu
+    @pytest.mark.parametrize("D", [64, 128])
+    @pytest.mark.parametrize("window", [0, 700])
+    def test_few_queries_in_splits(self, D, window):
+        """Long contexts beside short and empty ones, in parts that are merged."""
+        c = attention_case([3000, 30, 2500, 5, 5], [5, 8, 3, 2, 0], 8, 2, D, 160, window)
+        near(context(on(c, "cuda")), c, True)
+        c["ctx"][3] = 0  # no keys: zeros
+        d = on(c, "cuda")
+        got = context(d)
+        assert not got[16:18].any()
+        near(got, c, True)
+
     @pytest.mark.gpu
     def test_sequences_without_queries(self):
         c = attention_case([64, 100, 40], [0, 7, 0], 8, 2, 128, 130)
