@@ -90,10 +90,19 @@ __global__ void reshape_and_cache_fp8_kernel(
 // Infinities become +-448 * 2^e.
 //
 // A page's rows have to be known together, so the block of a page's first token in the
-// call (`own`) finds all of them by reading the whole slot map, 4 bytes a token out of
-// L2; the blocks of its other tokens end. Slots given twice take the later token's row.
+// call finds all of them by reading the whole slot map, 4 bytes a token out of L2; the
+// blocks of its other tokens leave it alone. Slots given twice take the later token's row.
 // A wave then takes a page of one KV head, K or V: up to 16 rows in registers, their
-// largest bits (bf16 magnitudes order as integers), and the bytes out.
+// largest bits (bf16 magnitudes order as integers), and the bytes out by the scaling
+// conversions, two numbers at a time. Of a page with one new row (a decode step's) it takes
+// four heads of 128 at once.
+//
+// Measured (8 KV heads of 128, us, on the GPU; K and V are read and written once at 4.9 TB/s
+// in brackets): 1 token 4.0, 256 tokens of as many sequences 4.7 (0.3), 1536 6.0 (2.0), 8
+// prompts of 1000 16.2 (10.3), 16 of 1000 26.0 (20.2). A few tokens are two memory accesses,
+// a barrier and one more; prompts are bound by how few pages they are (500, 16 waves each).
+// Before the one-row form, with a page's heads to a wave each, 1536 tokens took 15.4; with
+// conversions through fp32 and the map read token by token, prompts of 8 x 1000 took 43.
 struct ScaledWrite {
   const short* k;  // [T, Hkv, D], rows sk elements apart
   const short* v;
@@ -248,12 +257,72 @@ __device__ __forceinline__ void write_scaled_page(const ScaledWrite& p, const in
   if (lane == 0 && now != old_raw) *scale = (unsigned char)now;
 }
 
-// `per` (64 at most) consecutive tokens to a block; VEC: rows and the slot map are 16-byte
-// aligned
+// The same where `token` alone is written, to row `off`: a wave takes 64 / (D / 8) heads.
+template <int D, bool VEC>
+__device__ __forceinline__ void write_scaled_row(const ScaledWrite& p, int token, int off,
+                                                 long page, int task) {
+  constexpr int LPR = D / 8, HEADS = 64 / LPR;
+  const int lane = threadIdx.x & 63, col = lane % LPR * 8;
+  const int item = task * HEADS + lane / LPR;
+  const bool used = item < 2 * p.Hkv;
+  const bool is_v = item >= p.Hkv;
+  const int head = !used ? 0 : is_v ? item - p.Hkv : item;
+  const long at = page * p.Hkv + head;
+  unsigned char* scale = (is_v ? p.v_scale : p.k_scale) + at;
+  unsigned char* rows = (is_v ? p.v_cache : p.k_cache) + at * (ROWS * D) + col;
+  const short* from = (is_v ? p.v : p.k) + head * D + col + token * (is_v ? p.sv : p.sk);
+  const int old_raw = *scale;
+  uint4 x;
+  if constexpr (VEC) {
+    x = *reinterpret_cast<const uint4*>(from);
+  } else {
+    short8_t e;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) e[j] = from[j];
+    x = __builtin_bit_cast(uint4, e);
+  }
+  const ushort2_t two = largest8(x);
+  int top = max((int)two[0], (int)two[1]);
+  const bool special = __any(top >= INF);
+  if (special) {
+    top = 0;
+    const short8_t e = __builtin_bit_cast(short8_t, x);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) top = max(top, (e[j] & 0x7fff) >= INF ? 0 : e[j] & 0x7fff);
+  }
+#pragma unroll
+  for (int step = LPR / 2; step > 0; step >>= 1) top = max(top, __shfl_xor(top, step, 64));
+  const int need = max((top >> 7) - 8 + ((top & 0x7f) > 0x60 ? 1 : 0), LEAST_SCALE);
+  const int old = old_raw == NO_SCALE ? 0 : old_raw;
+  const int now = off == 0 ? need : max(old, need);
+  if (!used) return;
+  uint2 codes = encode8(x, now);
+  if (special) codes = encode_special8(x, codes);
+  if (off != 0 && now != old_raw) {
+    constexpr int AHEAD = 4;
+#pragma unroll 1
+    for (int r = 0; r < ROWS; r += AHEAD) {
+      uint2 kept[AHEAD];
+#pragma unroll
+      for (int i = 0; i < AHEAD; ++i)
+        kept[i] = *reinterpret_cast<const uint2*>(rows + (r + i) * D);
+#pragma unroll
+      for (int i = 0; i < AHEAD; ++i)
+        *reinterpret_cast<uint2*>(rows + (r + i) * D) =
+            old_raw == NO_SCALE ? no_numbers8(kept[i]) : rescale8(kept[i], max(old, 1), now);
+    }
+  }
+  *reinterpret_cast<uint2*>(rows + off * D) = codes;
+  if (lane % LPR == 0 && now != old_raw) *scale = (unsigned char)now;
+}
+
+// `per` (64 at most) consecutive tokens to a block, the pages that begin among them two at a
+// time; VEC: rows and the slot map are 16-byte aligned
 template <int D, bool VEC>
 __global__ __launch_bounds__(512, 6) void write_scaled_kernel(const ScaledWrite p, const int per) {
-  __shared__ int token_of[ROWS];
-  __shared__ int taken;  // an earlier token's block writes this page
+  constexpr int PAIR = 2;
+  __shared__ int token_of[PAIR][ROWS];
+  __shared__ int taken[PAIR];  // an earlier token's block writes this page
   const int wave = threadIdx.x >> 6, waves = blockDim.x >> 6, lane = threadIdx.x & 63;
   const int first = blockIdx.x * per;
   auto page_of = [&](int slot) { return (unsigned int)slot < p.limit ? slot >> 4 : -1; };
@@ -264,21 +333,31 @@ __global__ __launch_bounds__(512, 6) void write_scaled_kernel(const ScaledWrite 
   unsigned long todo = __ballot(lane < per && first + lane < p.T && page_here >= 0 &&
                                 page_here != page_before);
   while (todo) {
-    const int at = __builtin_ctzl(todo);
-    todo &= todo - 1;
-    const int t = first + at;
-    const int page = __builtin_amdgcn_readlane(page_here, at);
-    if (threadIdx.x < ROWS) token_of[threadIdx.x] = -1;
-    if (threadIdx.x == ROWS) taken = 0;
+    int t[PAIR], page[PAIR];
+#pragma unroll
+    for (int b = 0; b < PAIR; ++b) {
+      const int at = todo ? __builtin_ctzl(todo) : 0;
+      t[b] = first + at;
+      page[b] = todo ? __builtin_amdgcn_readlane(page_here, at) : -1;
+      todo &= todo - (todo ? 1 : 0);
+    }
+    if (threadIdx.x < PAIR * ROWS) token_of[threadIdx.x / ROWS][threadIdx.x % ROWS] = -1;
+    if (threadIdx.x < PAIR) taken[threadIdx.x] = 0;
     __syncthreads();
-    auto here = [&](int slot) { return (unsigned int)slot >> 4 == (unsigned int)page; };
+    auto here = [&](int slot) {
+      const unsigned int at = (unsigned int)slot >> 4;  // (negative: no page's)
+      return at == (unsigned int)page[0] || at == (unsigned int)page[1];
+    };
     auto look = [&](int j) {
       const int slot = p.slots[j];
-      if (!here(slot)) return;
-      if (j < t) taken = 1;
-      else atomicMax(&token_of[slot & (ROWS - 1)], j);
+#pragma unroll
+      for (int b = 0; b < PAIR; ++b) {
+        if ((unsigned int)slot >> 4 != (unsigned int)page[b]) continue;
+        if (j < t[b]) taken[b] = 1;
+        else atomicMax(&token_of[b][slot & (ROWS - 1)], j);
+      }
     };
-    // eight tokens at a time, looked at singly only where one of them is of this page
+    // eight tokens at a time, looked at singly only where one of them is of these pages
     const int whole = VEC ? p.T & ~7 : 0;
     for (int j = threadIdx.x * 8; j < whole; j += blockDim.x * 8) {
       const int4 a = *reinterpret_cast<const int4*>(p.slots + j);
@@ -291,10 +370,29 @@ __global__ __launch_bounds__(512, 6) void write_scaled_kernel(const ScaledWrite 
     }
     for (int j = whole + threadIdx.x; j < p.T; j += blockDim.x) look(j);
     __syncthreads();
-    if (!taken)
-      for (int task = blockIdx.y * waves + wave; task < 2 * p.Hkv; task += gridDim.y * waves)
-        write_scaled_page<D, VEC>(p, token_of, page, task);
-    __syncthreads();
+    // one row (a decode step's) or several: the pages' tasks one after the other
+    unsigned int given[PAIR];
+    int tasks[PAIR];
+#pragma unroll
+    for (int b = 0; b < PAIR; ++b) {
+      given[b] = (unsigned int)__ballot(lane < ROWS && token_of[b][lane % ROWS] >= 0) & 0xffff;
+      const bool one = (given[b] & (given[b] - 1)) == 0;
+      tasks[b] = given[b] == 0 || taken[b] ? 0 : one ? (2 * p.Hkv * (D / 8) + 63) / 64 : 2 * p.Hkv;
+    }
+    for (int task = blockIdx.y * waves + wave; task < tasks[0] + tasks[1];
+         task += gridDim.y * waves) {
+      const int b = task >= tasks[0];
+      const int of = b ? task - tasks[0] : task;
+      const unsigned int rows = b ? given[1] : given[0];
+      const int at = b ? page[1] : page[0];
+      if ((rows & (rows - 1)) == 0) {
+        const int off = __builtin_ctz(rows);
+        write_scaled_row<D, VEC>(p, token_of[b][off], off, at, of);
+      } else {
+        write_scaled_page<D, VEC>(p, token_of[b], at, of);
+      }
+    }
+    if (todo) __syncthreads();
   }
 }
 
@@ -323,9 +421,15 @@ extern "C" hipError_t ks_write_scaled_pages(const void* k, const void* v, void* 
                       (unsigned int)(pages < (1L << 27) ? pages * ROWS : 1L << 31),
                       sk,
                       sv};
-  const int per = T <= 1024 ? 1 : T >= 65536 ? 64 : (int)((T + 1023) / 1024);
+  // Tokens to a block, and blocks to a page's heads. One of eight waves, for two tokens each,
+  // up to what a decode step has (us, 1536 tokens of as many sequences / 2 prompts of 1000:
+  // so 6.0 / 11.0, two blocks 8.5 / 8.3, one for four tokens 8.0 / 8.4: steps are the more
+  // frequent); above, prompts (8 of 1000: about 1024 blocks 15.2, half as many 16.4, twice
+  // 19.5).
+  const int per = T <= 512 ? 1 : T <= 2048 ? 2 : T >= 65536 ? 64 : (int)((T + 1023) / 1024);
   // a page's heads, K and V, in blocks of up to eight waves
-  const long tasks = 2 * Hkv, parts = tasks <= 8 * 64 ? (tasks + 7) / 8 : 64;
+  const long tasks = 2 * Hkv;
+  const long parts = T <= 2048 ? 1 : tasks <= 8 * 64 ? (tasks + 7) / 8 : 64;
   const dim3 grid((unsigned)((T + per - 1) / per), (unsigned)parts);
   const dim3 block(64 * (unsigned)(tasks < 8 ? tasks : 8));
 #define GO(DD, VV) \
