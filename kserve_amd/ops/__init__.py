@@ -208,10 +208,11 @@ def paged_attention_decode(
             window,
         )
         return out
-    return torch_ref.paged_attention_decode(
+    got = torch_ref.paged_attention_decode(
         q, k_cache, v_cache, block_tables, context_lens, scale,
         window=window, k_scale=k_scale, v_scale=v_scale,
     )
+    return got if out is None else out.copy_(got)
 
 
 def flash_prefill_varlen(

@@ -100,7 +100,7 @@ __global__ __launch_bounds__(NW * 64, 4) void scaled_decode_kernel(const ScaledD
   // first pair does not depend on the context, its page ids are on the way before that is
   // known (entries behind the context are not used).
   int id = 0;
-  const bool known = p.n_splits == 1 && p.window == 0;
+  const bool known = p.n_splits == 1 && p.window == 0 && p.max_blocks > 0;
   if (known) id = bt[min(2 * (wave + (lane >> 1) * NW) + (lane & 1), p.max_blocks - 1)];
   const int ctx = context_of(p, s);
   const Range rg = page_range(ctx, p.window, 0, p.n_splits, NW);

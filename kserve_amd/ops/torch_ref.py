@@ -121,6 +121,10 @@ def reshape_and_cache(
 ) -> None:
     if k_scale is not None or v_scale is not None:
         check_scaled_pages(k_cache, v_cache, k_scale, v_scale)
+        if k.shape != v.shape or k.shape[1:] != (k_cache.shape[1], k_cache.shape[3]):
+            raise RuntimeError("reshape_and_cache: k and v [tokens, kv_heads, D] of the pages")
+        if slot_mapping.dim() != 1 or slot_mapping.shape[0] < k.shape[0]:
+            raise RuntimeError("slot_mapping: a vector of the tokens")
         write_scaled_pages(k, k_cache, k_scale, slot_mapping)
         write_scaled_pages(v, v_cache, v_scale, slot_mapping)
         return
@@ -156,6 +160,29 @@ def check_scaled_pages(k_cache, v_cache, k_scale, v_scale) -> None:
 def scaled_pages(cache: torch.Tensor, scale: torch.Tensor) -> torch.Tensor:
     """The values [pages, kv_heads, block, D] that a block-scaled cache holds, in fp32."""
     return torch.ldexp(cache.float(), (scale.view(torch.uint8).int() - 127)[..., None, None])
+
+
+def scaled_context(
+    q, k_cache, v_cache, k_scale, v_scale, block_tables, context_lens, window
+):
+    """What attention over block-scaled pages reads: (K, V as values, page ids inside the
+    cache, context lengths within their table rows)."""
+    check_scaled_pages(k_cache, v_cache, k_scale, v_scale)
+    pages, kv_heads, block, D = k_cache.shape
+    if q.dim() != 3 or q.shape[2] != D or pages < 1 or q.shape[1] % max(kv_heads, 1):
+        raise RuntimeError(
+            "scaled pages: queries [tokens, heads, D] of the pages' D, whole groups of "
+            "heads, a page at least"
+        )
+    if block_tables.dtype != torch.int32 or context_lens.dtype != torch.int32:
+        raise RuntimeError("scaled pages: block_tables and context_lens int32")
+    if window < 0:
+        raise RuntimeError("scaled pages: sizes out of range")
+    return (
+        scaled_pages(k_cache, k_scale), scaled_pages(v_cache, v_scale),
+        block_tables.clamp(0, pages - 1),
+        context_lens.clamp(0, block_tables.shape[1] * block),
+    )
 
 
 def write_scaled_pages(x, cache, scale, slot_mapping) -> None:
@@ -199,8 +226,9 @@ def paged_attention_decode(
     v_scale: Optional[torch.Tensor] = None,
 ) -> torch.Tensor:
     if k_scale is not None or v_scale is not None:
-        check_scaled_pages(k_cache, v_cache, k_scale, v_scale)
-        k_cache, v_cache = scaled_pages(k_cache, k_scale), scaled_pages(v_cache, v_scale)
+        k_cache, v_cache, block_tables, context_lens = scaled_context(
+            q, k_cache, v_cache, k_scale, v_scale, block_tables, context_lens, window
+        )
     num_seqs, num_heads, head_dim = q.shape
     num_kv_heads = k_cache.shape[1]
     block_size = k_cache.shape[2]
@@ -282,9 +310,11 @@ def context_attention_varlen(
 ) -> torch.Tensor:
     """Prefill attention against the paged cache (supports chunked prefill:
     new tokens attend to all cached tokens before them, causally)."""
-    if k_scale is not None or v_scale is not None:
-        check_scaled_pages(k_cache, v_cache, k_scale, v_scale)
-        k_cache, v_cache = scaled_pages(k_cache, k_scale), scaled_pages(v_cache, v_scale)
+    scaled = k_scale is not None or v_scale is not None
+    if scaled:
+        k_cache, v_cache, block_tables, context_lens = scaled_context(
+            q, k_cache, v_cache, k_scale, v_scale, block_tables, context_lens, window
+        )
     num_heads = q.shape[1]
     num_kv_heads = k_cache.shape[1]
     head_dim = q.shape[2]
@@ -314,6 +344,8 @@ def context_attention_varlen(
             bad |= pos_k <= pos_q - window
         scores.masked_fill_(bad.unsqueeze(0), float("-inf"))
         probs = torch.softmax(scores, dim=-1)
+        if scaled:  # queries that see no key give zeros
+            probs = probs.masked_fill(bad.all(dim=1)[None, :, None], 0.0)
         o = torch.einsum("hts,hsd->htd", probs, vals)
         out[a:b] = o.transpose(0, 1).to(q.dtype)
     return out

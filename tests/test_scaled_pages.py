@@ -332,16 +332,28 @@ class TestDecode:
         c["vs"].view(torch.uint8)[::2] = 140
         near(decode(on(c, dev)), c)
 
-    @pytest.mark.gpu
-    def test_empty_context_and_out(self):
+    @pytest.mark.parametrize("dev", devices())
+    @pytest.mark.parametrize("empty", [0, -3])
+    def test_empty_context_and_out(self, dev, empty):
         """A sequence without keys gives zeros; `out` is filled and returned."""
         c = attention_case([40, 1, 20], [1] * 3, 8, 2, 128, 60)
-        c["ctx"][1] = 0
-        d = on(c, "cuda")
+        c["ctx"][1] = empty
+        d = on(c, dev)
         out = torch.full_like(d["q"], 7.0)
         assert decode(d, out=out) is out
         assert not out[1].any()
+        c["ctx"][1] = 0
         near(out, c)
+
+    @pytest.mark.parametrize("dev", devices())
+    def test_tables_without_columns(self, dev):
+        """Nothing to read: zeros, whatever the lengths say."""
+        c = attention_case([40, 30], [1, 1], 8, 2, 64, 65)
+        d = on(c, dev)
+        d["table"] = d["table"][:, :0].contiguous()
+        assert not decode(d).any()
+        assert not context(d).any()
+        assert not context(d, 40).any()
 
     @pytest.mark.gpu
     def test_strided_queries_and_negative_scale(self):
@@ -353,11 +365,12 @@ class TestDecode:
         d["q"] = wide[:, 2:10]
         near(decode(d), c)
 
-    @pytest.mark.gpu
-    def test_ids_outside_the_cache(self):
+    @pytest.mark.parametrize("dev", devices())
+    @pytest.mark.parametrize("window", [0, 30])
+    def test_ids_outside_the_cache(self, dev, window):
         """Table entries and lengths out of range stay inside the cache."""
-        c = attention_case([40, 100], [1] * 2, 8, 2, 128, 80)
-        d = on(c, "cuda")
+        c = attention_case([40, 100], [1] * 2, 8, 2, 128, 80, window)
+        d = on(c, dev)
         d["table"][0, 1], d["table"][0, 2] = -5, 1 << 30
         d["ctx"][0] = 1 << 30
         got = decode(d)
@@ -414,15 +427,26 @@ class TestContext:
         assert not got[16:18].any()
         near(got, c, True)
 
+    @pytest.mark.parametrize("dev", devices())
+    @pytest.mark.parametrize("n", [3, 70])
+    def test_contexts_shorter_than_their_queries(self, dev, n):
+        """Queries ahead of the context's first token see nothing: zeros."""
+        c = attention_case([n, 90], [n, n], 8, 2, 64, 145)
+        c["ctx"][0] = n - 2
+        d = on(c, dev)
+        got = context(d)
+        assert not got[:2].any()
+        near(got, c, True)
+
     @pytest.mark.gpu
     def test_sequences_without_queries(self):
         c = attention_case([64, 100, 40], [0, 7, 0], 8, 2, 128, 130)
         near(context(on(c, "cuda")), c, True)
 
-    @pytest.mark.gpu
-    def test_ids_outside_the_cache(self):
+    @pytest.mark.parametrize("dev", devices())
+    def test_ids_outside_the_cache(self, dev):
         c = attention_case([40, 100], [9, 30], 8, 2, 128, 140)
-        d = on(c, "cuda")
+        d = on(c, dev)
         d["table"][0] = torch.tensor([-5, 1 << 30, 3] + [0] * (d["table"].shape[1] - 3))
         d["ctx"][0] = 1 << 30
         got = context(d)
@@ -554,6 +578,18 @@ class TestRefusals:
                 context(x)
             with pytest.raises(RuntimeError):
                 ops.reshape_and_cache(k, k, x["kc"], x["vc"], slots, k_scale=x["ks"], v_scale=x["vs"])
+        for bad in [
+            dict(q=c["q"][:, :3]), dict(q=c["q"][..., :32]), dict(table=c["table"].long()),
+            dict(ctx=c["ctx"].long()), dict(window=-1),
+            dict(kc=c["kc"][:0], vc=c["vc"][:0], ks=c["ks"][:0], vs=c["vs"][:0]),
+        ]:
+            with pytest.raises(RuntimeError):
+                decode(dict(c, **bad))
+            with pytest.raises(RuntimeError):
+                context(dict(c, **bad), 1)
+        for x, y, s in [(k, k[:, :1], slots), (k[..., :32], k[..., :32], slots), (k, k, slots[:0])]:
+            with pytest.raises(RuntimeError):
+                ops.reshape_and_cache(x, y, c["kc"], c["vc"], s, k_scale=c["ks"], v_scale=c["vs"])
 
     @pytest.mark.gpu
     def test_kernels_forms(self):
