@@ -21,6 +21,12 @@
 // The weights keep 24 bits as three bf16 parts, as in attention_decode.hip: in the 16
 // columns side by side for groups of up to five heads, by a second product for six to
 // eight.
+//
+// What bounds it: the pages. 256 sequences of 2048 +- 60% (32 / 8 heads of 128) take 186 us,
+// 5.8 TB/s, all of 2048 168 (6.4); the units' vector instructions are busy for a tenth of that
+// and their matrix cores for a tenth. 1 of 131071 under groups of eight 50 with the launch
+// that merges (5.3 TB/s); one of 560 8.1: four memory accesses one after the other, and the
+// sums.
 #include <type_traits>
 
 #include "mfma_attention.h"
@@ -78,6 +84,16 @@ __device__ __forceinline__ void add_parts(f32x4_t (&o)[N]) {
     }
 }
 
+// 16 bytes of K. With heads of 128 two loads take halves of the same lines, which have to
+// stay in the cache between them; other lines pass once (us, K kept and V passing / both
+// passing / both kept: 256 sequences of 2048 168 / 172 / 186, of 2048 +- 60% 186 / 195 / 203,
+// 1536 of 560 286 / 312 / 312; with heads of 64, whose loads take whole lines, 64 of 601
+// behind a window 7.4 / 7.1).
+template <int D>
+__device__ __forceinline__ uint4 load_k16(const char* from) {
+  return D > 64 ? *reinterpret_cast<const uint4*>(from) : load16_nt(from);
+}
+
 constexpr int BATCH = 32;  // pairs whose page ids and scales a wave fetches at once
 
 template <int D, int NW, bool WIDE>  // WIDE: groups of 6 to 8
@@ -96,12 +112,6 @@ __global__ __launch_bounds__(NW * 64, 4) void scaled_decode_kernel(const ScaledD
   const int lane = threadIdx.x & 63;
   const int* bt = p.block_tables + (long)s * p.max_blocks;
 
-  // Lane l of a batch from pair n on: page (l & 1) of pair n + l / 2 * NW. Where a wave's
-  // first pair does not depend on the context, its page ids are on the way before that is
-  // known (entries behind the context are not used).
-  int id = 0;
-  const bool known = p.n_splits == 1 && p.window == 0 && p.max_blocks > 0;
-  if (known) id = bt[min(2 * (wave + (lane >> 1) * NW) + (lane & 1), p.max_blocks - 1)];
   const int ctx = context_of(p, s);
   const Range rg = page_range(ctx, p.window, 0, p.n_splits, NW);
   const int n_lo = split * rg.per + wave;
@@ -116,16 +126,15 @@ __global__ __launch_bounds__(NW * 64, 4) void scaled_decode_kernel(const ScaledD
 
   __shared__ __attribute__((aligned(16))) char lds[NW][AREA];
 
+  // lane l of a batch from pair n on: page (l & 1) of pair n + l / 2 * NW
+  int id = 0;
   unsigned int ks = 0, vs = 0;
-  auto fetch_scales = [&]() {
+  auto fetch = [&](int n) {
+    id = bt[min(rg.first + 2 * (n + (lane >> 1) * NW) + (lane & 1), rg.last)];
     id = min(max(id, 0), p.s8.pages - 1);
     const long at = (long)id * p.Hkv + kvh;
     ks = p.s8.k[at];
     vs = p.s8.v[at];
-  };
-  auto fetch = [&](int n) {
-    id = bt[min(rg.first + 2 * (n + (lane >> 1) * NW) + (lane & 1), rg.last)];
-    fetch_scales();
   };
   uint4 kr[2][NI], vr[2][NI];
   const unsigned int klane = col * D + g * 16, vlane = lane * 16;
@@ -141,7 +150,7 @@ __global__ __launch_bounds__(NW * 64, 4) void scaled_decode_kernel(const ScaledD
     for (int h = 0; h < 2; ++h) {
       const char* from = tile(p.k_cache, i, h);
 #pragma unroll
-      for (int j = 0; j < NI; ++j) kr[h][j] = load16_nt(from + klane + j * 64);
+      for (int j = 0; j < NI; ++j) kr[h][j] = load_k16<D>(from + klane + j * 64);
     }
   };
   auto load_v = [&](int i) {
@@ -153,8 +162,7 @@ __global__ __launch_bounds__(NW * 64, 4) void scaled_decode_kernel(const ScaledD
     }
   };
   if (n_lo < n_hi) {
-    if (known) fetch_scales();
-    else fetch(n_lo);
+    fetch(n_lo);
     load_k(0);
     load_v(0);
   }
@@ -461,8 +469,7 @@ __global__ __launch_bounds__(NW * 64, NB == 1 ? 3 : 2) void scaled_few_kernel(co
     for (int h = 0; h < 2; ++h) {
       const char* from = tile(p.k_cache, i, h);
 #pragma unroll
-      for (int j = 0; j < NI; ++j)
-        kr[h][j] = *reinterpret_cast<const uint4*>(from + klane + j * 64);
+      for (int j = 0; j < NI; ++j) kr[h][j] = load_k16<D>(from + klane + j * 64);
     }
   };
   auto load_v = [&](int i) {
@@ -471,7 +478,7 @@ __global__ __launch_bounds__(NW * 64, NB == 1 ? 3 : 2) void scaled_few_kernel(co
       const char* from = tile(p.v_cache, i, h);
 #pragma unroll
       for (int j = 0; j < NI; ++j)
-        vr[h][j] = *reinterpret_cast<const uint4*>(from + vlane + j * 1024);
+        vr[h][j] = load16_nt(from + vlane + j * 1024);
     }
   };
   if (n_lo < n_hi) {
@@ -646,27 +653,27 @@ __global__ __launch_bounds__(NW * 64, NB == 1 ? 3 : 2) void scaled_few_kernel(co
   }
 }
 
-// Waves that share a context, 4 or 8, and its splits.
+// Waves that share a context, 4 or 8, and its splits (us; 8 KV heads of 128).
 //
-// From UNIT_BLOCKS blocks on, one to a compute unit, four waves and no splits (us, 4 x 1 / 8
-// x 1 / 4 waves x 2 splits, 8 KV heads of 128: 32 sequences of 1500 +- 60% 26.9 / 25.9 /
-// 29.9, 64 of 600 +- 50% 21.3 / 21.9 / 27.4, 96 of 3000 +- 60% 118 / 124 / 125, 256 of 100
-// 20 / 25 / 31, of 2048 +- 60% 199 / 197 / 218). Below, splits make up that many blocks (1
-// of 131071 under groups of eight 81 / 52 / 53 with 16, 32 and 64, of 7000 14.5 / 13.2 /
-// 15.1; 8 of 1500 17.5 / 14.4 / 14.7 with 2, 4 and 8), unless eight waves take a table in
-// SHORT pairs each, which spares the launch that merges (1 of 560 10.2, as 4 x 4 12.9; 1 of
-// 2000 20.1 and 12.3 as 4 x 16). Waves without a pair end at once (1000 of 16 tokens 42 ->
-// 23).
+// From TWO_BLOCKS blocks on, two to a compute unit, four waves and no splits (4 x 1 / 8 x 1 /
+// 4 waves x 2 splits: 64 sequences of 600 +- 50% 18.0 / 19.1 / 25.8, 96 of 3000 +- 60% 111 /
+// 114 / 120, 256 of 100 17.6 / 21.5, of 2048 +- 60% 189 / 184 / 206, 1000 of 16 21.7 / 35.0:
+// waves without a pair end at once, but their block's LDS keeps others out); from UNIT_BLOCKS
+// on eight (32 of 1500 +- 60% 24.6 / 21.5 / 27.1). Below, splits make up that many blocks (1
+// of 131071 under groups of eight 83 / 53 / 53 with 16, 32 and 64, of 7000 18.0 / 15.0 / 16.0
+// with 8, 16 and 32), unless eight waves take a table in SHORT pairs each, which spares the
+// launch that merges (8 of 1500 15.0, as 4 x 4 16.0; 1 of 560 9.1 and 14.8; 1 of 2000 16.1,
+// and 14.8 as 4 x 16).
 struct Shape {
   int waves, splits;
 };
-constexpr long UNIT_BLOCKS = 256, SHORT = 4;
+constexpr long UNIT_BLOCKS = 256, TWO_BLOCKS = 512, SHORT = 6;
 Shape decode_shape(long seqs, long kv_heads, long max_blocks) {
   const long blocks = seqs * kv_heads;
-  if (blocks <= 0 || blocks >= UNIT_BLOCKS) return {4, 1};
+  if (blocks <= 0 || blocks >= TWO_BLOCKS) return {4, 1};
   const long pairs = (max_blocks + 1) / 2;
   const long splits = (UNIT_BLOCKS + blocks / 2) / blocks;
-  if (pairs <= 8 * SHORT || splits == 1) return {8, 1};
+  if (pairs <= 8 * SHORT || splits <= 1) return {8, 1};
   const long most = (pairs + 3) / 4;  // a pair for every wave
   return {4, (int)(splits < most ? splits : most)};
 }
@@ -805,7 +812,7 @@ extern "C" int ks_scaled_few_splits(int num_seqs, int max_q_len, int Hq, int Hkv
   const int groups = (int)(((long)max_q_len * (Hq / Hkv) + 31) / 32);
   const long blocks = (long)num_seqs * Hkv * groups, pairs = (max_nb + 1) / 2;
   // (as for decode: a launch that merges costs what eight pairs of a wave take)
-  if (blocks <= 0 || blocks >= UNIT_BLOCKS || pairs <= 8 * SHORT) return 1;
+  if (blocks <= 0 || blocks >= UNIT_BLOCKS || pairs <= 4 * 8) return 1;
   long splits = (UNIT_BLOCKS + blocks / 2) / blocks;
   const long most = (pairs + 7) / 8;  // two pairs for every wave
   if (splits > most) splits = most;

@@ -320,7 +320,7 @@ class TestDecode:
          ([17] * 300, 8, 8), ([30] * 520, 4, 4), ([600] * 70, 8, 8)],
     )
     def test_splits_and_waves(self, D, lens, heads, kv):
-        """Contexts in one part and in several, launches of one, two and four waves."""
+        """Contexts in one part and in several, blocks of four and of eight waves."""
         c = attention_case(lens, [1] * len(lens), heads, kv, D, 40)
         near(decode(on(c, "cuda")), c)
 
