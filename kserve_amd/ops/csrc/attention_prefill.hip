@@ -36,6 +36,13 @@
 // bidirectional 20 / 17 us, 64 x 123 level at 13; fp32 scores, 4 x 2000, 16 / 4 heads
 // 239 / 223 us.
 //
+// Block-scaled E4M3 pages: a wave's 16 rows of a tile are one page, so its power of two is one
+// operand of the conversions that widen them between registers and LDS, and is applied
+// exactly. That widening is what they cost (2 x 1000 queries over 13000 keys, us: 430 to 510 by
+// box, bf16 pages 400 beside 510; without the conversions 435, without the LDS writes 460,
+// without both 410); K as bytes into the products that take E8M0 scales themselves was 5%
+// faster, but sums products in less than 32 bits. Few queries go to attention_scaled.hip.
+//
 // Replaces the vLLM flash prefill the reference delegates to. Numerics oracles:
 // ops/torch_ref.flash_prefill_varlen and context_attention_varlen.
 #include "mfma_attention.h"
