@@ -371,19 +371,26 @@ class ModelRunner:
 
         bs = self.config.cache.block_size
         computed = [r.num_computed_tokens for r in requests]
-        used = [-(-(c + n) // bs) for c, n in zip(computed, widths)]
-        lists = [block_manager.get_block_table(r)[:n] for r, n in zip(requests, used)]
-        ints = [
-            np.asarray([p for x in lists for p in x], dtype=np.int32),
-            np.cumsum([0] + [len(x) for x in lists], dtype=np.int32),
-            np.asarray(computed, dtype=np.int32),
-            np.asarray(widths, dtype=np.int32),
-        ]
-        out = self._to_device(list(arrays) + ints)
+        # page ids, where each request's begin, computed and new lengths: one array
+        ints, starts, widest = [], [0], 0
+        for r, c, n in zip(requests, computed, widths):
+            used = -(-(c + n) // bs)
+            table = block_manager.get_block_table(r)
+            if len(table) < used:
+                raise IndexError(f"request {r.request_id}: {len(table)} pages of {used}")
+            ints += table[:used]
+            starts.append(len(ints))
+            widest = max(widest, used)
+        P, S = len(ints), len(computed)
+        ints += starts
+        ints += computed
+        ints += widths
+        *out, packed = self._to_device([*arrays, np.array(ints, dtype=np.int32)])
+        pages, starts, computed, new = packed.split((P, S + 1, S, S))
         made = ops.build_paged_batch(
-            *out[len(arrays) :], sum(widths), max(used, default=0) if tables else 0, bs
+            pages, starts, computed, new, sum(widths), widest if tables else 0, bs
         )
-        return out[: len(arrays)], made
+        return out, made
 
     def _to_device(self, arrays) -> List[torch.Tensor]:
         """The arrays on the device. A GPU gets them in one copy out of pinned

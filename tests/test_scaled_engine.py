@@ -304,6 +304,9 @@ class TestRunnerTables:
         assert meta.block_tables.tolist() == [
             (manager.get_block_table(q)[:u] + [0] * max(used))[: max(used)] for q, u in zip(reqs, used)
         ]
+        reqs[1].num_computed_tokens = 90  # more than its pages hold
+        with pytest.raises(IndexError):
+            r.prepare_prefill(batch, manager)
         for q in reqs:
             q.num_computed_tokens = 0
         batch = ScheduledBatch(is_prefill=True, requests=reqs, num_scheduled_tokens=[3, 2, 1])
