@@ -284,7 +284,7 @@ class TestRunnerTables:
         manager = BlockManager(96, bs)
         reqs = []
         for i, (n, c) in enumerate([(40, 0), (33, 16), (70, 61)]):
-            q = Request(request_id=str(i), prompt_token_ids=list(range(n)),
+            q = Request(request_id=str(i), prompt_token_ids=list(range(200)),
                         sampling_params=SamplingParams(max_tokens=4))
             manager.allocate(q, n)
             q.num_computed_tokens = c
