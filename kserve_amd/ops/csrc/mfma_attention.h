@@ -310,8 +310,8 @@ __global__ __launch_bounds__(256, 2) void prefill_attention_kernel(
     return PAGED && SRC != PAGES_FP8S ? bt[group_of(t) >> 4] : 0;
   };
   // Block-scaled: ids and exponents of the wave's pages of 64 tiles, a tile to a lane. (As
-  // loads per tile they are waited for with that tile's rows behind them: 2 x 1000 queries
-  // over 13000 keys 545 us.)
+  // loads per tile they are waited for with that tile's rows behind them: us, so / per tile,
+  // 2 x 1000 queries over 13000 keys 510 / 545, 4 x 48 after 12900 79 / 84.)
   int ids = 0;
   unsigned int k_exps = 0, v_exps = 0;
   auto fetch_pages = [&](int t) {
