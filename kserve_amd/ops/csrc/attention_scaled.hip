@@ -22,8 +22,8 @@
 // columns side by side for groups of up to five heads, by a second product for six to
 // eight.
 //
-// What bounds it: the pages. 256 sequences of 2048 +- 60% (32 / 8 heads of 128) take 186 us,
-// 5.8 TB/s, all of 2048 168 (6.4); the units' vector instructions are busy for a tenth of that
+// What bounds it: the pages. 256 sequences of 2048 +- 60% (32 / 8 heads of 128) take 172 us,
+// 6.3 TB/s, the longest first; the units' vector instructions are busy for a tenth of that
 // and their matrix cores for a tenth. 1 of 131071 under groups of eight 50 with the launch
 // that merges (5.3 TB/s); one of 560 8.1: four memory accesses one after the other, and the
 // sums.
@@ -50,11 +50,78 @@ struct ScaledDecode {
   float* part_out;  // [S, H, n_splits, D]
   float* part_ml;   // [S, H, n_splits, 2]
   int window;
+  int sorted;  // keys of a sequence from which on the longest go first, or 0
 };
 
 // keys of sequence s: as many as its table row has at most
 __device__ __forceinline__ int context_of(const ScaledDecode& p, int s) {
   return min(p.ctx_lens[s], p.max_blocks * PAGE);
+}
+
+// The sequence, and its keys, that block row r of `seqs` takes: of the last LAST rows the
+// longest first, to an eighth of its length, so that the launch does not end in one that
+// begins late. Every wave finds it by itself, which takes a microsecond: lane l holds the
+// lengths of rows l, l + 64, .., and each bit of them, from the highest on, leaves the rows
+// that have it or the rest. Where no row reads p.sorted keys nothing is moved.
+//
+// us, in order / so: one query each, 64 of 2048 +- 60% 51.4 / 48.9, 96 of 3000 +- 60% 105 /
+// 95, 160 of 2048 +- 60% 124 / 112, 256 of 2048 +- 60% 188 / 172 and all of 2048 170 / 171,
+// 512 of 600 +- 60% 109 / 107, 1536 of 560 286 / 287, 256 of 100 in wide tables 17.8 / 18.4;
+// five queries, 64 of 1500 +- 60% 41.4 / 41.0, 96 61 / 58 and all of 1500 58 / 60, 192 120 /
+// 110, 256 of 800 +- 60% 78.5 / 81.
+constexpr int LAST = 256;
+__device__ __forceinline__ int2 longest_first(const ScaledDecode& p, int r, int seqs, int lane) {
+  const int first = max(seqs - LAST, 0);
+  if (r < first) return int2{r, context_of(p, r)};
+  constexpr int N = LAST / 64;
+  constexpr int LOW = 20, BITS = 6;  // of a float: exponent, 3 bits behind it
+  constexpr int BASE = (127 + 9) << 3;  // 512's
+  int len[N], key[N];
+  bool some = false;
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    const int s = first + i * 64 + lane;
+    len[i] = context_of(p, min(s, seqs - 1));
+    const int reads = p.window > 0 ? min(len[i], p.window) : len[i];
+    some |= reads >= p.sorted;
+    const int of = (__builtin_bit_cast(int, (float)max(reads, 1)) >> LOW) - BASE;
+    key[i] = min(max(of, 0), (1 << BITS) - 1);
+  }
+  int at = r - first;
+  if (__any(some)) {
+    unsigned long long left[N];
+#pragma unroll
+    for (int i = 0; i < N; ++i) left[i] = __ballot(first + i * 64 + lane < seqs);
+    int rank = at;
+#pragma unroll
+    for (int bit = BITS - 1; bit >= 0; --bit) {
+      unsigned long long with[N];
+      int n = 0;
+#pragma unroll
+      for (int i = 0; i < N; ++i) {
+        with[i] = left[i] & __ballot(key[i] >> bit & 1);
+        n += __popcll(with[i]);
+      }
+      const bool in = rank < n;
+      rank -= in ? 0 : n;
+#pragma unroll
+      for (int i = 0; i < N; ++i) left[i] = in ? with[i] : left[i] & ~with[i];
+    }
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const int n = __popcll(left[i]);
+      if (rank >= 0 && rank < n) {
+        const int before = (int)__popcll(left[i] & ((1ull << lane) - 1));
+        at = i * 64 + __ffsll(__ballot((left[i] >> lane & 1) && before == rank)) - 1;
+      }
+      rank -= n;
+    }
+  }
+  at = __builtin_amdgcn_readfirstlane(at);
+  int ctx = len[0];
+#pragma unroll
+  for (int i = 1; i < N; ++i) ctx = at >> 6 == i ? len[i] : ctx;
+  return int2{first + at, __builtin_amdgcn_readlane(ctx, at & 63)};
 }
 
 // 16-byte chunk that chunk c of staged row r is XORed with: the 16 rows of both pages
@@ -107,12 +174,14 @@ __global__ __launch_bounds__(NW * 64, 4) void scaled_decode_kernel(const ScaledD
   constexpr int MERGE = 8 * (D + 4) + 16;  // floats: sums of 8 heads, their m and l
   constexpr int AREA = MERGE * 4 > 2 * TILE ? MERGE * 4 : 2 * TILE;
 
-  const int kvh = blockIdx.x, s = blockIdx.y, split = blockIdx.z;
+  const int kvh = blockIdx.x, split = blockIdx.z;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int lane = threadIdx.x & 63;
+  const int2 of = p.sorted ? longest_first(p, blockIdx.y, gridDim.y, lane)
+                           : int2{(int)blockIdx.y, context_of(p, blockIdx.y)};
+  const int s = of.x, ctx = of.y;
   const int* bt = p.block_tables + (long)s * p.max_blocks;
 
-  const int ctx = context_of(p, s);
   const Range rg = page_range(ctx, p.window, 0, p.n_splits, NW);
   const int n_lo = split * rg.per + wave;
   const int n_hi = min((split + 1) * rg.per, rg.pairs);
@@ -407,15 +476,17 @@ __global__ __launch_bounds__(NW * 64, NB == 1 ? 3 : 2) void scaled_few_kernel(co
   const ScaledDecode& p = f.d;
 
   const int kvh = blockIdx.x % p.Hkv, first_col = blockIdx.x / p.Hkv * COLS;
-  const int s = blockIdx.y, split = blockIdx.z;
+  const int split = blockIdx.z;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int lane = threadIdx.x & 63;
+  const int2 of = p.sorted ? longest_first(p, blockIdx.y, gridDim.y, lane)
+                           : int2{(int)blockIdx.y, context_of(p, blockIdx.y)};
+  const int s = of.x, ctx = of.y;
   const int G = p.group;
   const int q_start = min(max(f.cu_q[s], 0), f.tokens);
   const int q_len = min(f.cu_q[s + 1], f.tokens) - q_start;
   const int cols = min(q_len * G - first_col, COLS);  // of the block
   if (cols <= 0) return;
-  const int ctx = context_of(p, s);
   const int start = ctx - q_len;  // position of query 0
   auto low = [&](int pos) { return pos > 0 ? low_of(pos, p.window, 0) : 0; };
   // keys of the block's first and last query
@@ -656,8 +727,8 @@ __global__ __launch_bounds__(NW * 64, NB == 1 ? 3 : 2) void scaled_few_kernel(co
 // Waves that share a context, 4 or 8, and its splits (us; 8 KV heads of 128).
 //
 // From TWO_BLOCKS blocks on, two to a compute unit, four waves and no splits (4 x 1 / 8 x 1 /
-// 4 waves x 2 splits: 64 sequences of 600 +- 50% 18.0 / 19.1 / 25.8, 96 of 3000 +- 60% 111 /
-// 114 / 120, 256 of 100 17.6 / 21.5, of 2048 +- 60% 189 / 184 / 206, 1000 of 16 21.7 / 35.0:
+// 4 waves x 2 splits: 64 sequences of 600 +- 50% 18.5 / 19.7 / 23.6, 96 of 3000 +- 60% 95 /
+// 95 / 108, 256 of 100 17.8 / 21.6 / 21.5, of 2048 +- 60% 172 / 172 / 205, 1000 of 16 21.8 / 34.8:
 // waves without a pair end at once, but their block's LDS keeps others out); from UNIT_BLOCKS
 // on eight (32 of 1500 +- 60% 24.6 / 21.5 / 27.1). Below, splits make up that many blocks (1
 // of 131071 under groups of eight 83 / 53 / 53 with 16, 32 and 64, of 7000 18.0 / 15.0 / 16.0
@@ -668,6 +739,15 @@ struct Shape {
   int waves, splits;
 };
 constexpr long UNIT_BLOCKS = 256, TWO_BLOCKS = 512, SHORT = 6;
+
+// From which length of a sequence on a launch takes the longest first: blocks that all
+// begin at once are left in order, and tables that hold no such sequence.
+constexpr int LONG = 512, FEW_LONG = 1536;
+int sorted_from(int length, long blocks, int splits, int max_blocks, int window) {
+  const long reads = (long)max_blocks * PAGE;
+  const bool any = (window > 0 && window < reads ? window : reads) >= length;
+  return splits == 1 && blocks >= TWO_BLOCKS && any ? length : 0;
+}
 Shape decode_shape(long seqs, long kv_heads, long max_blocks) {
   const long blocks = seqs * kv_heads;
   if (blocks <= 0 || blocks >= TWO_BLOCKS) return {4, 1};
@@ -740,7 +820,9 @@ extern "C" hipError_t ks_paged_attention_decode_scaled(
                        splits,
                        (float*)part_out,
                        (float*)part_ml,
-                       window};
+                       window,
+                       sorted_from(LONG, (long)num_seqs * num_kv_heads, splits, max_blocks,
+                                   window)};
   if (head_dim == 128) return launch_scaled<128>(p, num_seqs, waves, stream);
   if (head_dim == 64) return launch_scaled<64>(p, num_seqs, waves, stream);
   return hipErrorInvalidValue;
@@ -767,6 +849,10 @@ extern "C" hipError_t ks_scaled_few(
     const void* ctx_lens, const void* cu_q, int num_seqs, int max_q_len, int Hq, int Hkv,
     int head_dim, int max_nb, int pages, float scale, long sq, int window, long rows,
     int n_splits, void* part_out, void* part_ml, hipStream_t stream) {
+  const int nb = Hkv > 0 ? ks_scaled_few_columns(max_q_len, Hq / Hkv) : 0;
+  if (nb == 0) return hipErrorInvalidValue;
+  if (num_seqs == 0) return hipSuccess;
+  const int groups = (max_q_len * (Hq / Hkv) + 16 * nb - 1) / (16 * nb);
   const ScaledDecode d{out,
                        (const short*)q,
                        (const unsigned char*)k_cache,
@@ -784,12 +870,10 @@ extern "C" hipError_t ks_scaled_few(
                        n_splits,
                        nullptr,
                        nullptr,
-                       window};
+                       window,
+                       sorted_from(FEW_LONG, (long)num_seqs * Hkv * groups, n_splits, max_nb,
+                                   window)};
   const FewArgs f{d, (const int*)cu_q, (int)(rows / Hq), (float*)part_out, (float*)part_ml};
-  const int nb = ks_scaled_few_columns(max_q_len, Hq / Hkv);
-  if (nb == 0) return hipErrorInvalidValue;
-  if (num_seqs == 0) return hipSuccess;
-  const int groups = (max_q_len * (Hq / Hkv) + 16 * nb - 1) / (16 * nb);
   const dim3 grid(Hkv * groups, num_seqs, n_splits);
 #define GO(DD, BB) \
   hipLaunchKernelGGL((scaled_few_kernel<DD, 4, BB>), grid, dim3(256), 0, stream, f)

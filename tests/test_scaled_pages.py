@@ -324,6 +324,22 @@ class TestDecode:
         c = attention_case(lens, [1] * len(lens), heads, kv, D, 40)
         near(decode(on(c, "cuda")), c)
 
+    @pytest.mark.gpu
+    @pytest.mark.parametrize("window", [0, 600])
+    @pytest.mark.parametrize(
+        "S, longest",
+        [(64, 511), (64, 512), (65, 900), (200, 700), (256, 4000), (257, 700), (330, 600)],
+    )
+    def test_sequences_of_many_lengths(self, S, longest, window):
+        """Long sequences among short, equal and empty ones, whichever goes first."""
+        g = torch.Generator().manual_seed(S)
+        lens = torch.randint(0, 200, (S,), generator=g)
+        at = torch.randperm(S, generator=g)[: max(3, 8000 // longest)]
+        lens[at] = torch.randint(longest // 2, longest + 1, (len(at),), generator=g)
+        lens[at[0]], lens[at[1]], lens[0], lens[S - 1] = longest, longest, 0, longest - 1
+        c = attention_case(lens.tolist(), [1] * S, 8, 8, 64, 45, window)
+        near(decode(on(c, "cuda")), c)
+
     @pytest.mark.parametrize("dev", devices())
     def test_extreme_scales(self, dev):
         """Pages from 2^-90 to 2^13 beside one another."""
@@ -426,6 +442,23 @@ class TestContext:
         got = context(d)
         assert not got[16:18].any()
         near(got, c, True)
+
+    @pytest.mark.gpu
+    @pytest.mark.parametrize("window", [0, 1600])
+    @pytest.mark.parametrize(
+        "S, longest, most",
+        [(64, 1535, 4), (64, 1536, 4), (65, 3100, 40), (257, 1800, 9), (300, 1600, 16)],
+    )
+    def test_few_queries_of_many_lengths(self, S, longest, most, window):
+        """Long sequences among short ones and ones without queries."""
+        g = torch.Generator().manual_seed(S)
+        new = torch.randint(0, most + 1, (S,), generator=g)
+        lens = new + torch.randint(0, 60, (S,), generator=g)
+        at = torch.randperm(S, generator=g)[:5]
+        lens[at] = torch.randint(longest // 2, longest + 1, (5,), generator=g)
+        new[at[0]], lens[at[0]], lens[at[1]] = most, longest, longest
+        c = attention_case(lens.tolist(), new.tolist(), 8, 8, 64, 165, window)
+        near(context(on(c, "cuda")), c, True)
 
     @pytest.mark.parametrize("dev", devices())
     @pytest.mark.parametrize("n", [3, 70])
