@@ -6,15 +6,18 @@
 //
 // One launch: the blocks of the first part take TOKENS tokens each and find their
 // requests by the sums of the lengths, which every block forms by itself, 1024 at a time
-// in LDS (cheaper than a launch that forms them once: 64 blocks of 1024 lengths read
-// 256 KB out of L2); the blocks of the second part take TABLE table entries each.
+// (cheaper than a launch that forms them once: 64 blocks of 1024 lengths read 256 KB out
+// of L2); the blocks of the second part take ENTRIES table entries each (four times as
+// many one after the other: 96 requests' tables of 130 pages 5.2 to 9.2 us). What bounds
+// it: the launch and three dependent reads (96 requests of 5 tokens 4.1 us), with 1024
+// tables of 8101 pages the 55 MB (10.6 us, 5.2 TB/s).
 #include "common.h"
 
 namespace {
 
-constexpr int TOKENS = 1024;  // of a block, 4 to a thread
-constexpr int TABLE = 4096;   // entries of a block, in steps of 4 to a thread
-constexpr int CHUNK = 1024;   // requests whose sums are in LDS at a time
+constexpr int TOKENS = 1024;   // of a block, 4 to a thread
+constexpr int ENTRIES = 1024;  // of the tables, the same
+constexpr int CHUNK = 1024;    // requests whose sums a block forms at a time
 
 struct BatchArgs {
   const int* pages;        // [P] requests' pages one after the other
@@ -38,127 +41,167 @@ __device__ __forceinline__ int2 page_span(const BatchArgs& p, int s) {
   return int2{a, b - a};
 }
 
+// f over the lanes up to and with this one
+template <typename F>
+__device__ __forceinline__ unsigned int lanes_up_to(unsigned int x, unsigned int none, F f) {
+#define FROM(ctrl, rows) \
+  x = f(x, (unsigned int)__builtin_amdgcn_update_dpp((int)none, (int)x, ctrl, rows, 15, false))
+  FROM(0x111, 15);  // lanes of a row of 16 by 1, 2, 4 and 8
+  FROM(0x112, 15);
+  FROM(0x114, 15);
+  FROM(0x118, 15);
+  FROM(0x142, 10);  // the last lane of rows 0 and 2 to the next
+  FROM(0x143, 12);  // lane 31 to the upper half
+#undef FROM
+  return x;
+}
+
+// Every request marks its first token among the block's in LDS; a scan over the marks then
+// gives each token its request (a search for each among the sums: 96 requests 5.7 for 4.1
+// us, 1024 of a token 8.8 for 6.1; one request 3.1 for 3.6).
 __device__ void token_part(const BatchArgs& p) {
-  // first token of each of a chunk's requests, and the end of the last
-  __shared__ long sums[CHUNK + 1];
-  __shared__ long part[4];
+  __shared__ __attribute__((aligned(16))) int owner[TOKENS];  // request that begins here, or -1
+  __shared__ unsigned int part[2][4], first_begin;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const long t0 = (long)blockIdx.x * TOKENS + threadIdx.x * 4;
-  long pos[4] = {0, 0, 0, 0};
-  int slot[4] = {-1, -1, -1, -1}, seq[4] = {-1, -1, -1, -1};
-  long base = 0;
-  for (int s0 = 0; s0 < p.S; s0 += CHUNK) {
-    long len[4], mine = 0;
+  const unsigned int T = p.T, t_block = blockIdx.x * (unsigned int)TOKENS;
+  const unsigned int t0 = t_block + threadIdx.x * 4;
+  *reinterpret_cast<int4*>(owner + threadIdx.x * 4) = int4{-1, -1, -1, -1};
+  // sums stop at 2^32 - 1: no token is behind them
+  auto add = [](unsigned int a, unsigned int b) { return __builtin_elementwise_add_sat(a, b); };
+  unsigned int base = 0;
+  int turn = 0;
+  for (int s0 = 0; s0 < p.S; s0 += CHUNK, turn ^= 1) {
+    const int s = s0 + threadIdx.x * 4;
+    unsigned int len[4], mine = 0;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      const int s = s0 + threadIdx.x * 4 + i;
-      len[i] = s < p.S ? max(p.fresh[s], 0) : 0;
-      mine += len[i];
+      len[i] = s + i < p.S ? max(p.fresh[s + i], 0) : 0;
+      mine = add(mine, len[i]);
     }
-    long up = mine;  // inclusive over the wave
-#pragma unroll
-    for (int off = 1; off < 64; off <<= 1) {
-      const long x = __shfl_up(up, off, 64);
-      if (lane >= off) up += x;
-    }
-    if (lane == 63) part[wave] = up;
+    const unsigned int up = lanes_up_to(mine, 0, add);
+    if (lane == 63) part[turn][wave] = up;
     __syncthreads();
-    long at = base + up - mine;
-    for (int w = 0; w < wave; ++w) at += part[w];
+    unsigned int at = base;
+#pragma unroll
+    for (int w = 0; w < 4; ++w) {
+      if (w < wave) at = add(at, part[turn][w]);
+      base = add(base, part[turn][w]);
+    }
+    const unsigned int before = __shfl_up(up, 1, 64);
+    if (lane > 0) at = add(at, before);
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      sums[threadIdx.x * 4 + i] = at;
-      at += len[i];
-    }
-    if (threadIdx.x == 255) sums[CHUNK] = at;
-    __syncthreads();
-    const int n = min(CHUNK, p.S - s0);
-    const long end = sums[n];
-    if (blockIdx.x == 0) {
-      for (int i = threadIdx.x; i < n; i += 256)
-        p.cu[s0 + i] = (int)min(sums[i], (long)p.T);
-      if (s0 + n == p.S && threadIdx.x == 0) p.cu[p.S] = (int)min(end, (long)p.T);
-    }
-    if (t0 + 4 > base && t0 < end) {
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const long t = t0 + i;
-        if (t < base || t >= end || t >= p.T) continue;
-        int lo = 0, hi = n;  // the last request that begins at or before t
-        while (hi - lo > 1) {
-          const int mid = (lo + hi) >> 1;
-          if (sums[mid] <= t) lo = mid;
-          else hi = mid;
-        }
-        const int s = s0 + lo;
-        const unsigned int at_pos =
-            (unsigned int)max(p.computed[s], 0) + (unsigned int)(t - sums[lo]);
-        const unsigned int j = at_pos / (unsigned int)p.block;
-        const int2 span = page_span(p, s);
-        pos[i] = at_pos;
-        seq[i] = s;
-        if (j < (unsigned int)span.y) {
-          const long at_slot =
-              (long)p.pages[span.x + j] * p.block + (at_pos - j * (unsigned int)p.block);
-          if (at_slot >= 0 && at_slot <= 0x7fffffffL) slot[i] = (int)at_slot;
-        }
+      const unsigned int end = add(at, len[i]);
+      if (end > t_block && at < t_block + TOKENS && len[i] > 0) {
+        owner[at > t_block ? at - t_block : 0] = s + i;
+        if (at <= t_block) first_begin = at;
       }
+      if (blockIdx.x == 0 && s + i < p.S) p.cu[s + i] = (int)min(at, T);
+      at = end;
     }
-    base = sums[CHUNK];
-    __syncthreads();  // before the next chunk's sums
-    if (base > t0 - threadIdx.x * 4 + TOKENS && blockIdx.x != 0) break;
+    if (base >= t_block + TOKENS && blockIdx.x != 0) break;
   }
-  if (p.S == 0 && blockIdx.x == 0 && threadIdx.x == 0) p.cu[0] = 0;
+  if (blockIdx.x == 0 && threadIdx.x == 0) p.cu[p.S] = (int)min(base, T);
+  __syncthreads();
+
+  const int4 marks = *reinterpret_cast<const int4*>(owner + threadIdx.x * 4);
+  const int mark[4] = {marks.x, marks.y, marks.z, marks.w};
+  unsigned int from[4], run = 0;  // 1 + where the token's request is marked
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    if (mark[i] >= 0) run = threadIdx.x * 4 + i + 1;
+    from[i] = run;
+  }
+  auto most = [](unsigned int a, unsigned int b) { return max(a, b); };
+  const unsigned int up = lanes_up_to(run, 0, most);
+  if (lane == 63) part[0][wave] = up;
+  __syncthreads();
+  const unsigned int left = __shfl_up(up, 1, 64);
+  unsigned int carry = lane > 0 ? left : 0;
+#pragma unroll
+  for (int w = 0; w < 3; ++w)
+    if (w < wave) carry = max(carry, part[0][w]);
+
+  // four tokens in step, so that their reads are under way together
+  int s[4], id[4];
+  int2 span[4];
+  unsigned int at_pos[4], page[4];
+  bool in[4], held[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    from[i] = max(from[i], carry);
+    in[i] = from[i] > 0 && t0 + i < min(base, T);
+    s[i] = in[i] ? owner[from[i] - 1] : 0;
+    const unsigned int begin = from[i] > 1 ? t_block + from[i] - 1 : first_begin;
+    at_pos[i] = t0 + i - begin;
+    span[i] = int2{0, 0};
+    if (in[i]) {
+      at_pos[i] += (unsigned int)max(p.computed[s[i]], 0);
+      span[i] = page_span(p, s[i]);
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    page[i] = at_pos[i] / (unsigned int)p.block;
+    held[i] = in[i] && page[i] < (unsigned int)span[i].y;
+    id[i] = 0;
+    if (held[i]) id[i] = p.pages[span[i].x + page[i]];
+  }
 #pragma unroll
   for (int i = 0; i < 4; ++i)
-    if (t0 + i < p.T) {
-      p.positions[t0 + i] = pos[i];
-      p.slots[t0 + i] = slot[i];
-      p.seqs[t0 + i] = seq[i];
+    if (t0 + i < T) {
+      const long slot = (long)id[i] * p.block + (at_pos[i] - page[i] * (unsigned int)p.block);
+      p.positions[t0 + i] = in[i] ? at_pos[i] : 0;
+      p.slots[t0 + i] = held[i] && slot >= 0 && slot <= 0x7fffffffL ? (int)slot : -1;
+      p.seqs[t0 + i] = in[i] ? s[i] : -1;
     }
 }
 
 __device__ void table_part(const BatchArgs& p) {
   const unsigned int total = (unsigned int)p.S * p.width;  // below 2^31
-  const unsigned int first = (blockIdx.x - p.token_blocks) * (unsigned int)TABLE;
-  for (int step = 0; step < TABLE; step += 1024) {
-    const unsigned int at = first + step + threadIdx.x * 4;
-    if (at >= total) break;
-    int s = (int)(at / p.width), c = (int)(at - s * (unsigned int)p.width);
-    auto held_of = [&](int2 span) {
-      const long ctx = (long)max(p.computed[s], 0) + max(p.fresh[s], 0);
-      return (int)min((ctx + p.block - 1) / p.block, (long)span.y);
-    };
-    int2 span = page_span(p, s);
-    int held = held_of(span);
-    int4 id{0, 0, 0, 0};
-    if (c + 4 <= p.width) {  // of one row; at a multiple of 4 bytes only
-      if (c + 4 <= held) __builtin_memcpy(&id, p.pages + span.x + c, 16);
-      else if (c < held) {
-        id.x = p.pages[span.x + c];
-        if (c + 1 < held) id.y = p.pages[span.x + c + 1];
-        if (c + 2 < held) id.z = p.pages[span.x + c + 2];
-      }
-    } else {
-      int one[4] = {0, 0, 0, 0};
+  const unsigned int at =
+      (blockIdx.x - p.token_blocks) * (unsigned int)ENTRIES + threadIdx.x * 4;
+  if (at >= total) return;
+  int s = (int)(at / p.width), c = (int)(at - s * (unsigned int)p.width);
+  auto held_of = [&](int row, int2 span) {
+    const long ctx = (long)max(p.computed[row], 0) + max(p.fresh[row], 0);
+    return (int)min((ctx + p.block - 1) / p.block, (long)span.y);
+  };
+  int4 id{0, 0, 0, 0};
+  if (c + 4 <= p.width) {  // of one row; at a multiple of 4 bytes only
+    const int2 span = page_span(p, s);
+    const int held = held_of(s, span);
+    if (c + 4 <= held) __builtin_memcpy(&id, p.pages + span.x + c, 16);
+    else if (c < held) {
+      id.x = p.pages[span.x + c];
+      if (c + 1 < held) id.y = p.pages[span.x + c + 1];
+      if (c + 2 < held) id.z = p.pages[span.x + c + 2];
+    }
+  } else {
+    int from[4], one[4];
+    bool any[4];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        if (at + i >= total) continue;
-        if (c < held) one[i] = p.pages[span.x + c];
-        if (++c == p.width && ++s < p.S) {
-          c = 0;
-          span = page_span(p, s);
-          held = held_of(span);
-        }
+    for (int i = 0; i < 4; ++i) {
+      const int2 span = page_span(p, s);
+      any[i] = c < held_of(s, span) && at + i < total;
+      from[i] = span.x + c;
+      if (++c == p.width && s + 1 < p.S) {
+        c = 0;
+        ++s;
       }
-      id = int4{one[0], one[1], one[2], one[3]};
     }
-    if (at + 4 <= total) {
-      *reinterpret_cast<int4*>(p.tables + at) = id;
-    } else {
-      const int one[4] = {id.x, id.y, id.z, id.w};
-      for (unsigned int i = 0; i < 3 && at + i < total; ++i) p.tables[at + i] = one[i];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      one[i] = 0;
+      if (any[i]) one[i] = p.pages[from[i]];
     }
+    id = int4{one[0], one[1], one[2], one[3]};
+  }
+  if (at + 4 <= total) {
+    *reinterpret_cast<int4*>(p.tables + at) = id;
+  } else {
+    const int one[4] = {id.x, id.y, id.z, id.w};
+    for (unsigned int i = 0; i < 3 && at + i < total; ++i) p.tables[at + i] = one[i];
   }
 }
 
@@ -184,7 +227,7 @@ extern "C" hipError_t ks_paged_batch(const void* pages, const void* page_starts,
     return hipErrorInvalidValue;
   // one block of tokens at least: it writes cu_seqlens
   const int token_blocks = T > TOKENS ? (int)((T + TOKENS - 1) / TOKENS) : 1;
-  const int table_blocks = (int)((S * width + TABLE - 1) / TABLE);
+  const int table_blocks = (int)((S * width + ENTRIES - 1) / ENTRIES);
   const BatchArgs p{(const int*)pages, (const int*)page_starts, (const int*)computed,
                     (const int*)fresh, (long*)positions, (int*)slots, (int*)seqs, (int*)cu,
                     (int*)tables, (int*)ctx, (int)P, (int)S, (int)T, (int)width, (int)block,
