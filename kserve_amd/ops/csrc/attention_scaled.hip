@@ -51,6 +51,8 @@ struct ScaledDecode {
   float* part_ml;   // [S, H, n_splits, 2]
   int window;
   int sorted;  // keys of a sequence from which on the longest go first, or 0
+  int seqs;
+  int help;    // rows of blocks ahead of the sequences' that help with long ones, or 0
 };
 
 // keys of sequence s: as many as its table row has at most
@@ -124,6 +126,65 @@ __device__ __forceinline__ int2 longest_first(const ScaledDecode& p, int r, int 
   return int2{first + at, __builtin_amdgcn_readlane(ctx, at & 63)};
 }
 
+// Rows of blocks that help sequences much longer than the rest of a batch: one for every
+// 2^n pairs past the first 2^n, which are HELP_PAIRS and twice the mean at least, given out
+// in the order of the sequences for as long as there are any. Parts of a sequence lie at its
+// helpers' rows, the first at p.help + its first helper's. Up to LAST sequences, and where
+// the tables hold one that long: the launch that merges costs 3 us (us, without / with: 255
+// of 500 and one of 32768 257 / 66, one of 8192 89 / 61, 99 and one of 32768 243 / 52, 31 and
+// one 170 / 39; 256 of 500 in tables of 32768 48.0 / 50.8, 32 of 1500 19.8 / 22.6).
+constexpr int HELP = 24, HELP_PAIRS = 128;
+struct Helpers {
+  int first[LAST / 64], count[LAST / 64];  // of sequence 64 i + lane
+  __device__ __forceinline__ Helpers(const ScaledDecode& p, int lane) {
+    unsigned int pairs[LAST / 64], total = 0;
+#pragma unroll
+    for (int i = 0; i < LAST / 64; ++i) {
+      const int s = i * 64 + lane;
+      pairs[i] = page_range(context_of(p, min(s, p.seqs - 1)), p.window, 0, 1, 1).pairs;
+      if (s >= p.seqs) pairs[i] = 0;
+      total += pairs[i];
+    }
+    auto add = [](unsigned int a, unsigned int b) { return a + b; };
+    auto last = [](unsigned int x) { return (unsigned int)__builtin_amdgcn_readlane(x, 63); };
+    total = last(lanes_up_to(total, 0, add));
+    const unsigned int cut = max((unsigned int)HELP_PAIRS, 2 * (total / p.seqs));
+    const int shift = 32 - __builtin_clz(cut - 1);
+    unsigned int given = 0;
+#pragma unroll
+    for (int i = 0; i < LAST / 64; ++i) {
+      const unsigned int n = pairs[i] > 0 ? min((pairs[i] - 1) >> shift, (unsigned int)HELP) : 0;
+      const unsigned int up = lanes_up_to(n, 0, add);
+      first[i] = given + up - n;
+      count[i] = max(min((int)n, p.help - first[i]), 0);
+      given += last(up);
+    }
+  }
+  // the sequence for which `is` holds of its first helper and their number, or -1
+  template <typename F>
+  __device__ __forceinline__ int find(F is) const {
+    int s = -1;
+#pragma unroll
+    for (int i = 0; i < LAST / 64; ++i) {
+      const unsigned long long those = __ballot(is(first[i], count[i]));
+      if (those) s = i * 64 + __ffsll(those) - 1;
+    }
+    return __builtin_amdgcn_readfirstlane(s);
+  }
+  // {first, count} of sequence s
+  __device__ __forceinline__ int2 of(int s) const {
+    int at = 0, n = 0;  // (each by itself: a choice among members would be in memory)
+#pragma unroll
+    for (int i = 0; i < LAST / 64; ++i) {
+      const int a = __builtin_amdgcn_readlane(first[i], s & 63);
+      const int b = __builtin_amdgcn_readlane(count[i], s & 63);
+      at = s >> 6 == i ? a : at;
+      n = s >> 6 == i ? b : n;
+    }
+    return int2{at, n};
+  }
+};
+
 // 16-byte chunk that chunk c of staged row r is XORed with: the 16 rows of both pages
 // that half a wave's transposing load brings lie in different banks
 template <int D>
@@ -174,15 +235,36 @@ __global__ __launch_bounds__(NW * 64, 4) void scaled_decode_kernel(const ScaledD
   constexpr int MERGE = 8 * (D + 4) + 16;  // floats: sums of 8 heads, their m and l
   constexpr int AREA = MERGE * 4 > 2 * TILE ? MERGE * 4 : 2 * TILE;
 
-  const int kvh = blockIdx.x, split = blockIdx.z;
+  const int kvh = blockIdx.x, row = blockIdx.y;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int lane = threadIdx.x & 63;
-  const int2 of = p.sorted ? longest_first(p, blockIdx.y, gridDim.y, lane)
-                           : int2{(int)blockIdx.y, context_of(p, blockIdx.y)};
-  const int s = of.x, ctx = of.y;
+  int s = row - p.help, ctx = 0, split = blockIdx.z;
+  if (s < 0) {
+    const Helpers helpers(p, lane);
+    s = helpers.find([&](int first, int n) { return first <= row && row < first + n; });
+    if (s < 0) return;
+    ctx = context_of(p, s);
+  } else if (p.sorted) {
+    const int2 of = longest_first(p, s, p.seqs, lane);
+    s = of.x;
+    ctx = of.y;
+  } else {
+    ctx = context_of(p, s);
+  }
   const int* bt = p.block_tables + (long)s * p.max_blocks;
 
-  const Range rg = page_range(ctx, p.window, 0, p.n_splits, NW);
+  Range rg = page_range(ctx, p.window, 0, p.n_splits, NW);
+  long part_at = (long)s * p.H * p.n_splits + split, part_step = p.n_splits;  // by head
+  if (p.help > 0) {
+    const int2 helpers = Helpers(p, lane).of(s);
+    if (helpers.y > 0) {
+      split = row < p.help ? row - helpers.x + 1 : 0;
+      rg.splits = 1 + helpers.y;
+      rg.per = (rg.pairs + helpers.y) / rg.splits;
+      part_at = (long)(split > 0 ? row : p.help + helpers.x) * p.H;
+      part_step = 1;
+    }
+  }
   const int n_lo = split * rg.per + wave;
   const int n_hi = min((split + 1) * rg.per, rg.pairs);
   // waves with work, the first at least: the others end here and no barrier waits for them
@@ -404,7 +486,7 @@ __global__ __launch_bounds__(NW * 64, 4) void scaled_decode_kernel(const ScaledD
     if (rg.splits == 1) {
       store4(p.out, ((long)s * p.H + head) * D + d, acc * (sum > 0.f ? 1.f / sum : 0.f), 0);
     } else {
-      const long at = ((long)s * p.H + head) * p.n_splits + split;
+      const long at = part_at + head * part_step;
       *reinterpret_cast<f32x4_t*>(p.part_out + at * D + d) = acc;
       if (d == 0) {
         p.part_ml[at * 2] = top;
@@ -414,29 +496,41 @@ __global__ __launch_bounds__(NW * 64, 4) void scaled_decode_kernel(const ScaledD
   }
 }
 
-// Adds the splits of a (sequence, head): four waves take every fourth one, in order.
-// Sequences that one split covers are done.
+// Adds the splits of a (sequence, head), or of one with helpers: four waves take every
+// fourth one, in order. Sequences that one split covers are done.
 template <int D>
 __global__ __launch_bounds__(256) void scaled_decode_reduce_kernel(const ScaledDecode p,
                                                                    const int waves) {
   constexpr int ACC = D / 64;
-  const int h = blockIdx.x, s = blockIdx.y;
-  const Range rg = page_range(context_of(p, s), p.window, 0, p.n_splits, waves);
-  if (rg.splits == 1) return;
+  const int h = blockIdx.x;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  int s = blockIdx.y, splits;
+  if (p.help > 0) {
+    const Helpers helpers(p, lane);
+    const int row = s;
+    s = helpers.find([&](int first, int n) { return first == row && n > 0; });
+    if (s < 0) return;
+    splits = 1 + helpers.of(s).y;
+  } else {
+    splits = page_range(context_of(p, s), p.window, 0, p.n_splits, waves).splits;
+  }
+  if (splits == 1) return;
   const long sh = (long)s * p.H + h;
-  const float* ml = p.part_ml + sh * p.n_splits * 2;
+  auto at = [&](int sp) {
+    if (p.help == 0) return sh * p.n_splits + sp;
+    return (long)(blockIdx.y + (sp > 0 ? sp - 1 : p.help)) * p.H + h;
+  };
   float m = -3.4e38f;
-  for (int sp = lane; sp < rg.splits; sp += 64) m = fmaxf(m, ml[sp * 2]);
+  for (int sp = lane; sp < splits; sp += 64) m = fmaxf(m, p.part_ml[at(sp) * 2]);
   m = wave_reduce_max(m);
   float l = 0.f, acc[ACC];
 #pragma unroll
   for (int a = 0; a < ACC; ++a) acc[a] = 0.f;
 #pragma unroll 4
-  for (int sp = wave; sp < rg.splits; sp += 4) {
-    const float w = __builtin_amdgcn_exp2f(ml[sp * 2] - m);
-    l += w * ml[sp * 2 + 1];
-    const float* po = p.part_out + (sh * p.n_splits + sp) * D + lane * ACC;
+  for (int sp = wave; sp < splits; sp += 4) {
+    const float w = __builtin_amdgcn_exp2f(p.part_ml[at(sp) * 2] - m);
+    l += w * p.part_ml[at(sp) * 2 + 1];
+    const float* po = p.part_out + at(sp) * D + lane * ACC;
 #pragma unroll
     for (int a = 0; a < ACC; ++a) acc[a] += w * po[a];
   }
@@ -479,7 +573,7 @@ __global__ __launch_bounds__(NW * 64, NB == 1 ? 3 : 2) void scaled_few_kernel(co
   const int split = blockIdx.z;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int lane = threadIdx.x & 63;
-  const int2 of = p.sorted ? longest_first(p, blockIdx.y, gridDim.y, lane)
+  const int2 of = p.sorted ? longest_first(p, blockIdx.y, p.seqs, lane)
                            : int2{(int)blockIdx.y, context_of(p, blockIdx.y)};
   const int s = of.x, ctx = of.y;
   const int G = p.group;
@@ -736,9 +830,10 @@ __global__ __launch_bounds__(NW * 64, NB == 1 ? 3 : 2) void scaled_few_kernel(co
 // launch that merges (8 of 1500 15.0, as 4 x 4 16.0; 1 of 560 9.1 and 14.8; 1 of 2000 16.1,
 // and 14.8 as 4 x 16).
 struct Shape {
-  int waves, splits;
+  int waves, splits, help;
 };
 constexpr long UNIT_BLOCKS = 256, TWO_BLOCKS = 512, SHORT = 6;
+constexpr long HELP_READS = 8192;
 
 // From which length of a sequence on a launch takes the longest first: blocks that all
 // begin at once are left in order, and tables that hold no such sequence.
@@ -748,14 +843,19 @@ int sorted_from(int length, long blocks, int splits, int max_blocks, int window)
   const bool any = (window > 0 && window < reads ? window : reads) >= length;
   return splits == 1 && blocks >= TWO_BLOCKS && any ? length : 0;
 }
-Shape decode_shape(long seqs, long kv_heads, long max_blocks) {
+Shape decode_shape(long seqs, long kv_heads, long max_blocks, int window) {
   const long blocks = seqs * kv_heads;
-  if (blocks <= 0 || blocks >= TWO_BLOCKS) return {4, 1};
+  const long reads = max_blocks * PAGE;
+  const int help = blocks >= UNIT_BLOCKS && seqs <= LAST &&
+                           (window > 0 && window < reads ? window : reads) >= HELP_READS
+                       ? HELP
+                       : 0;
+  if (blocks <= 0 || blocks >= TWO_BLOCKS) return {4, 1, help};
   const long pairs = (max_blocks + 1) / 2;
   const long splits = (UNIT_BLOCKS + blocks / 2) / blocks;
-  if (pairs <= 8 * SHORT || splits <= 1) return {8, 1};
+  if (pairs <= 8 * SHORT || splits <= 1) return {8, 1, splits <= 1 ? help : 0};
   const long most = (pairs + 3) / 4;  // a pair for every wave
-  return {4, (int)(splits < most ? splits : most)};
+  return {4, (int)(splits < most ? splits : most), 0};
 }
 
 template <int D, int NW>
@@ -768,13 +868,13 @@ void launch_waves(const ScaledDecode& p, dim3 grid, hipStream_t stream) {
 
 template <int D>
 hipError_t launch_scaled(const ScaledDecode& p, int seqs, int waves, hipStream_t stream) {
-  const dim3 grid(p.Hkv, seqs, p.n_splits);
+  const dim3 grid(p.Hkv, p.help + seqs, p.n_splits);
   if (waves == 8) launch_waves<D, 8>(p, grid, stream);
   else launch_waves<D, 4>(p, grid, stream);
   HIP_CHECK_KERNEL();
-  if (p.n_splits > 1) {
-    hipLaunchKernelGGL((scaled_decode_reduce_kernel<D>), dim3(p.H, seqs), dim3(256), 0,
-                       stream, p, waves);
+  if (p.n_splits > 1 || p.help > 0) {
+    hipLaunchKernelGGL((scaled_decode_reduce_kernel<D>),
+                       dim3(p.H, p.help > 0 ? p.help : seqs), dim3(256), 0, stream, p, waves);
     HIP_CHECK_KERNEL();
   }
   return hipSuccess;
@@ -782,13 +882,15 @@ hipError_t launch_scaled(const ScaledDecode& p, int seqs, int waves, hipStream_t
 
 }  // namespace
 
-// waves | splits << 8 for such a call
-extern "C" int ks_scaled_decode_shape(int num_seqs, int num_kv_heads, int max_blocks) {
-  const Shape s = decode_shape(num_seqs, num_kv_heads, max_blocks);
-  return s.waves | s.splits << 8;
+// waves | splits << 8 | rows of helpers << 24 for such a call
+extern "C" int ks_scaled_decode_shape(int num_seqs, int num_kv_heads, int max_blocks,
+                                      int window) {
+  const Shape s = decode_shape(num_seqs, num_kv_heads, max_blocks, window);
+  return s.waves | s.splits << 8 | s.help << 24;
 }
 
-// part_out and part_ml are read where the shape has several splits
+// part_out [S, H, splits, D] and part_ml [S, H, splits, 2] where the shape has several
+// splits, [2 rows, H, D] and [2 rows, H, 2] where it has helpers
 extern "C" hipError_t ks_paged_attention_decode_scaled(
     void* out, const void* q, const void* k_cache, const void* v_cache,
     const void* k_scale, const void* v_scale, const void* block_tables,
@@ -799,8 +901,10 @@ extern "C" hipError_t ks_paged_attention_decode_scaled(
     return hipErrorInvalidValue;
   const int group = num_heads / num_kv_heads;
   const int waves = shape & 255;
-  const int splits = part_out && part_ml ? shape >> 8 : 1;
-  if (group < 1 || group > 8 || splits < 1 || (waves != 4 && waves != 8))
+  const bool parts = part_out && part_ml;
+  const int splits = parts ? shape >> 8 & 0xffff : 1, help = parts ? shape >> 24 : 0;
+  if (group < 1 || group > 8 || splits < 1 || (help > 0 && splits > 1) ||
+      (help > 0 && num_seqs > LAST) || (waves != 4 && waves != 8))
     return hipErrorInvalidValue;
   if (num_seqs == 0) return hipSuccess;
   const ScaledDecode p{out,
@@ -822,7 +926,9 @@ extern "C" hipError_t ks_paged_attention_decode_scaled(
                        (float*)part_ml,
                        window,
                        sorted_from(LONG, (long)num_seqs * num_kv_heads, splits, max_blocks,
-                                   window)};
+                                   window),
+                       num_seqs,
+                       help};
   if (head_dim == 128) return launch_scaled<128>(p, num_seqs, waves, stream);
   if (head_dim == 64) return launch_scaled<64>(p, num_seqs, waves, stream);
   return hipErrorInvalidValue;
@@ -872,7 +978,9 @@ extern "C" hipError_t ks_scaled_few(
                        nullptr,
                        window,
                        sorted_from(FEW_LONG, (long)num_seqs * Hkv * groups, n_splits, max_nb,
-                                   window)};
+                                   window),
+                       num_seqs,
+                       0};
   const FewArgs f{d, (const int*)cu_q, (int)(rows / Hq), (float*)part_out, (float*)part_ml};
   const dim3 grid(Hkv * groups, num_seqs, n_splits);
 #define GO(DD, BB) \

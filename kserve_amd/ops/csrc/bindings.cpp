@@ -43,7 +43,7 @@ hipError_t ks_paged_attention_decode_scaled(void*, const void*, const void*, con
                                             const void*, float, int, int, int, int, int,
                                             int, long, int, void*, void*, int,
                                             hipStream_t);
-int ks_scaled_decode_shape(int, int, int);
+int ks_scaled_decode_shape(int, int, int, int);
 int ks_context_scaled_splits(int, long, int, int, int, int, int);
 hipError_t ks_context_prefill_scaled(void*, const void*, const void*, const void*,
                                      const void*, const void*, const void*, const void*,
@@ -320,14 +320,15 @@ void paged_attention_decode_scaled(at::Tensor& out, at::Tensor& q, at::Tensor& k
   TORCH_CHECK(H / Hkv <= 8, "scaled pages: groups of up to 8 heads in decode");
   const c10::DeviceGuard guard(q.device());
   const int max_blocks = block_tables.size(1);
-  const int shape = ks_scaled_decode_shape(S, Hkv, max_blocks);
-  const int n_splits = shape >> 8;
+  const int shape = ks_scaled_decode_shape(S, Hkv, max_blocks, (int)window);
+  const int n_splits = shape >> 8 & 0xffff, help = shape >> 24;
   at::Tensor part_out, part_ml;
   void *po = nullptr, *pml = nullptr;
-  if (n_splits > 1) {
+  if (n_splits > 1 || help > 0) {
     auto opts = at::TensorOptions().dtype(at::kFloat).device(q.device());
-    part_out = at::empty({S, H, n_splits, D}, opts);
-    part_ml = at::empty({S, H, n_splits, 2}, opts);
+    const int64_t parts = help > 0 ? 2 * help : (int64_t)S * n_splits;
+    part_out = at::empty({parts, H, D}, opts);
+    part_ml = at::empty({parts, H, 2}, opts);
     po = part_out.data_ptr();
     pml = part_ml.data_ptr();
   }

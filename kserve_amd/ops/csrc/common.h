@@ -54,6 +54,21 @@ __device__ __forceinline__ float wave_reduce_max(float v) {
   return v;
 }
 
+// f over the lanes up to and with this one
+template <typename F>
+__device__ __forceinline__ unsigned int lanes_up_to(unsigned int x, unsigned int none, F f) {
+#define FROM(ctrl, rows) \
+  x = f(x, (unsigned int)__builtin_amdgcn_update_dpp((int)none, (int)x, ctrl, rows, 15, false))
+  FROM(0x111, 15);  // lanes of a row of 16 by 1, 2, 4 and 8
+  FROM(0x112, 15);
+  FROM(0x114, 15);
+  FROM(0x118, 15);
+  FROM(0x142, 10);  // the last lane of rows 0 and 2 to the next
+  FROM(0x143, 12);  // lane 31 to the upper half
+#undef FROM
+  return x;
+}
+
 // reduce within contiguous groups of `width` lanes (width = power of 2 <= 64)
 template <int WIDTH>
 __device__ __forceinline__ float group_reduce_sum(float v) {

@@ -41,21 +41,6 @@ __device__ __forceinline__ int2 page_span(const BatchArgs& p, int s) {
   return int2{a, b - a};
 }
 
-// f over the lanes up to and with this one
-template <typename F>
-__device__ __forceinline__ unsigned int lanes_up_to(unsigned int x, unsigned int none, F f) {
-#define FROM(ctrl, rows) \
-  x = f(x, (unsigned int)__builtin_amdgcn_update_dpp((int)none, (int)x, ctrl, rows, 15, false))
-  FROM(0x111, 15);  // lanes of a row of 16 by 1, 2, 4 and 8
-  FROM(0x112, 15);
-  FROM(0x114, 15);
-  FROM(0x118, 15);
-  FROM(0x142, 10);  // the last lane of rows 0 and 2 to the next
-  FROM(0x143, 12);  // lane 31 to the upper half
-#undef FROM
-  return x;
-}
-
 // Every request marks its first token among the block's in LDS; a scan over the marks then
 // gives each token its request (a search for each among the sums: 96 requests 5.7 for 4.1
 // us, 1024 of a token 8.8 for 6.1; one request 3.1 for 3.6).

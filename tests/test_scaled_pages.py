@@ -340,6 +340,24 @@ class TestDecode:
         c = attention_case(lens.tolist(), [1] * S, 8, 8, 64, 45, window)
         near(decode(on(c, "cuda")), c)
 
+    @pytest.mark.gpu
+    @pytest.mark.parametrize(
+        "S, long, heads, kv, D, window",
+        [(32, [8192], 8, 8, 64, 0), (40, [40000, 9000], 16, 8, 64, 0), (64, [12000], 8, 8, 128, 0),
+         (200, [4097, 8300], 8, 4, 64, 0), (256, [9000] * 30, 4, 4, 64, 0), (256, [8191, 100000], 4, 2, 64, 0),
+         (257, [9000], 2, 2, 64, 0), (70, [20000, 30000], 64, 8, 64, 8200), (64, [9000] * 64, 8, 8, 64, 0)],
+    )
+    def test_long_sequences_among_short(self, S, long, heads, kv, D, window):
+        """Some so long that other blocks take parts of them, as many as there are."""
+        g = torch.Generator().manual_seed(S)
+        lens = torch.randint(0, 120, (S,), generator=g)
+        lens[torch.randperm(S, generator=g)[: len(long)]] = torch.tensor(long)
+        c = attention_case(lens.tolist(), [1] * S, heads, kv, D, 46, window)
+        d = on(c, "cuda")
+        got = decode(d)
+        near(got, c)
+        assert torch.equal(got, decode(d))
+
     @pytest.mark.parametrize("dev", devices())
     def test_extreme_scales(self, dev):
         """Pages from 2^-90 to 2^13 beside one another."""
