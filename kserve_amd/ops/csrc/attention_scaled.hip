@@ -46,7 +46,7 @@ struct ScaledDecode {
   float scale;
   int H, Hkv, group, max_blocks;
   long sq;
-  int n_splits;
+  int n_splits, base;  // most, and those of any context that is long enough
   float* part_out;  // [S, H, n_splits, D]
   float* part_ml;   // [S, H, n_splits, 2]
   int window;
@@ -58,6 +58,18 @@ struct ScaledDecode {
 // keys of sequence s: as many as its table row has at most
 __device__ __forceinline__ int context_of(const ScaledDecode& p, int s) {
   return min(p.ctx_lens[s], p.max_blocks * PAGE);
+}
+
+// Splits of a context: p.base with a pair for every wave at least, or more of PART pairs
+constexpr int PART = 128;
+__device__ __forceinline__ Range decode_range(const ScaledDecode& p, int ctx, int waves) {
+  Range r = page_range(ctx, p.window, 0, p.base, waves);
+  const int more = min(r.pairs / PART, p.n_splits);
+  if (more > r.splits) {
+    r.splits = more;
+    r.per = (r.pairs + more - 1) / more;
+  }
+  return r;
 }
 
 // The sequence, and its keys, that block row r of `seqs` takes: of the last LAST rows the
@@ -127,13 +139,13 @@ __device__ __forceinline__ int2 longest_first(const ScaledDecode& p, int r, int 
 }
 
 // Rows of blocks that help sequences much longer than the rest of a batch: one for every
-// 2^n pairs past the first 2^n, which are HELP_PAIRS and twice the mean at least, given out
+// 2^n pairs past the first 2^n, which are PART and twice the mean at least, given out
 // in the order of the sequences for as long as there are any. Parts of a sequence lie at its
 // helpers' rows, the first at p.help + its first helper's. Up to LAST sequences, and where
 // the tables hold one that long: the launch that merges costs 3 us (us, without / with: 255
 // of 500 and one of 32768 257 / 66, one of 8192 89 / 61, 99 and one of 32768 243 / 52, 31 and
 // one 170 / 39; 256 of 500 in tables of 32768 48.0 / 50.8, 32 of 1500 19.8 / 22.6).
-constexpr int HELP = 24, HELP_PAIRS = 128;
+constexpr int HELP = 24;
 struct Helpers {
   int first[LAST / 64], count[LAST / 64];  // of sequence 64 i + lane
   __device__ __forceinline__ Helpers(const ScaledDecode& p, int lane) {
@@ -148,7 +160,7 @@ struct Helpers {
     auto add = [](unsigned int a, unsigned int b) { return a + b; };
     auto last = [](unsigned int x) { return (unsigned int)__builtin_amdgcn_readlane(x, 63); };
     total = last(lanes_up_to(total, 0, add));
-    const unsigned int cut = max((unsigned int)HELP_PAIRS, 2 * (total / p.seqs));
+    const unsigned int cut = max((unsigned int)PART, 2 * (total / p.seqs));
     const int shift = 32 - __builtin_clz(cut - 1);
     unsigned int given = 0;
 #pragma unroll
@@ -249,11 +261,13 @@ __global__ __launch_bounds__(NW * 64, 4) void scaled_decode_kernel(const ScaledD
     s = of.x;
     ctx = of.y;
   } else {
+    // (where few contexts have all splits, theirs are turned on to units of their own)
+    if (p.n_splits > p.base) s = (s + 5 * split + split / 8) % p.seqs;
     ctx = context_of(p, s);
   }
   const int* bt = p.block_tables + (long)s * p.max_blocks;
 
-  Range rg = page_range(ctx, p.window, 0, p.n_splits, NW);
+  Range rg = decode_range(p, ctx, NW);
   long part_at = (long)s * p.H * p.n_splits + split, part_step = p.n_splits;  // by head
   if (p.help > 0) {
     const int2 helpers = Helpers(p, lane).of(s);
@@ -512,7 +526,7 @@ __global__ __launch_bounds__(256) void scaled_decode_reduce_kernel(const ScaledD
     if (s < 0) return;
     splits = 1 + helpers.of(s).y;
   } else {
-    splits = page_range(context_of(p, s), p.window, 0, p.n_splits, waves).splits;
+    splits = decode_range(p, context_of(p, s), waves).splits;
   }
   if (splits == 1) return;
   const long sh = (long)s * p.H + h;
@@ -829,11 +843,16 @@ __global__ __launch_bounds__(NW * 64, NB == 1 ? 3 : 2) void scaled_few_kernel(co
 // with 8, 16 and 32), unless eight waves take a table in SHORT pairs each, which spares the
 // launch that merges (8 of 1500 15.0, as 4 x 4 16.0; 1 of 560 9.1 and 14.8; 1 of 2000 16.1,
 // and 14.8 as 4 x 16).
+//
+// Long contexts among short ones: without splits there are helpers; with them, up to
+// WIDE_SPLITS for the contexts that have PART pairs for each (us, without / with: one of
+// 32768 and 15 of 500 125 / 42, 23 170 / 38 with helpers, 7 67 / 40; 16 of 2048 in wide
+// tables 18.0 / 18.2).
 struct Shape {
-  int waves, splits, help;
+  int waves, base, splits, help;
 };
 constexpr long UNIT_BLOCKS = 256, TWO_BLOCKS = 512, SHORT = 6;
-constexpr long HELP_READS = 8192;
+constexpr long HELP_READS = 8192, WIDE_SPLITS = 16;
 
 // From which length of a sequence on a launch takes the longest first: blocks that all
 // begin at once are left in order, and tables that hold no such sequence.
@@ -845,17 +864,18 @@ int sorted_from(int length, long blocks, int splits, int max_blocks, int window)
 }
 Shape decode_shape(long seqs, long kv_heads, long max_blocks, int window) {
   const long blocks = seqs * kv_heads;
-  const long reads = max_blocks * PAGE;
-  const int help = blocks >= UNIT_BLOCKS && seqs <= LAST &&
-                           (window > 0 && window < reads ? window : reads) >= HELP_READS
-                       ? HELP
-                       : 0;
-  if (blocks <= 0 || blocks >= TWO_BLOCKS) return {4, 1, help};
+  const long reads = window > 0 && window < max_blocks * PAGE ? window : max_blocks * PAGE;
+  const int help = seqs > 0 && seqs <= LAST && reads >= HELP_READS ? HELP : 0;
+  if (blocks <= 0 || blocks >= TWO_BLOCKS) return {4, 1, 1, help};
   const long pairs = (max_blocks + 1) / 2;
-  const long splits = (UNIT_BLOCKS + blocks / 2) / blocks;
-  if (pairs <= 8 * SHORT || splits <= 1) return {8, 1, splits <= 1 ? help : 0};
+  long splits = (UNIT_BLOCKS + blocks / 2) / blocks;
+  if (splits <= 1) return {8, 1, 1, help};
+  if (pairs <= 8 * SHORT) return {8, 1, 1, 0};
   const long most = (pairs + 3) / 4;  // a pair for every wave
-  return {4, (int)(splits < most ? splits : most), 0};
+  splits = splits < most ? splits : most;
+  const long whole = reads / (2 * PAGE) / PART;
+  const long parts = whole < WIDE_SPLITS ? whole : WIDE_SPLITS;
+  return {4, (int)splits, (int)(splits < parts ? parts : splits), 0};
 }
 
 template <int D, int NW>
@@ -902,6 +922,7 @@ extern "C" hipError_t ks_paged_attention_decode_scaled(
   const int group = num_heads / num_kv_heads;
   const int waves = shape & 255;
   const bool parts = part_out && part_ml;
+  const int base = decode_shape(num_seqs, num_kv_heads, max_blocks, window).base;
   const int splits = parts ? shape >> 8 & 0xffff : 1, help = parts ? shape >> 24 : 0;
   if (group < 1 || group > 8 || splits < 1 || (help > 0 && splits > 1) ||
       (help > 0 && num_seqs > LAST) || (waves != 4 && waves != 8))
@@ -922,6 +943,7 @@ extern "C" hipError_t ks_paged_attention_decode_scaled(
                        max_blocks,
                        q_row_stride,
                        splits,
+                       base < splits ? base : splits,
                        (float*)part_out,
                        (float*)part_ml,
                        window,
@@ -973,6 +995,7 @@ extern "C" hipError_t ks_scaled_few(
                        Hq / Hkv,
                        max_nb,
                        sq,
+                       n_splits,
                        n_splits,
                        nullptr,
                        nullptr,

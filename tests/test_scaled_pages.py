@@ -345,6 +345,8 @@ class TestDecode:
         "S, long, heads, kv, D, window",
         [(32, [8192], 8, 8, 64, 0), (40, [40000, 9000], 16, 8, 64, 0), (64, [12000], 8, 8, 128, 0),
          (200, [4097, 8300], 8, 4, 64, 0), (256, [9000] * 30, 4, 4, 64, 0), (256, [8191, 100000], 4, 2, 64, 0),
+         (1, [70000], 8, 8, 64, 0), (4, [70000, 8200], 8, 8, 64, 0), (15, [33000], 8, 8, 128, 0),
+         (20, [9000, 30000], 16, 8, 64, 0), (22, [9000], 8, 8, 64, 0), (7, [30000], 8, 8, 64, 9000),
          (257, [9000], 2, 2, 64, 0), (70, [20000, 30000], 64, 8, 64, 8200), (64, [9000] * 64, 8, 8, 64, 0)],
     )
     def test_long_sequences_among_short(self, S, long, heads, kv, D, window):
