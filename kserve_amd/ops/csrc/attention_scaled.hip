@@ -841,8 +841,8 @@ __global__ __launch_bounds__(NW * 64, NB == 1 ? 3 : 2) void scaled_few_kernel(co
 // on eight (32 of 1500 +- 60% 24.6 / 21.5 / 27.1). Below, splits make up that many blocks (1
 // of 131071 under groups of eight 83 / 53 / 53 with 16, 32 and 64, of 7000 18.0 / 15.0 / 16.0
 // with 8, 16 and 32), unless eight waves take a table in SHORT pairs each, which spares the
-// launch that merges (8 of 1500 15.0, as 4 x 4 16.0; 1 of 560 9.1 and 14.8; 1 of 2000 16.1,
-// and 14.8 as 4 x 16).
+// launch that merges (eight waves / splits: 1 of 1500 13.7 / 9.3, 8 of 1500 13.9 / 10.7, 20
+// of 1000 12.0 / 15.1; 1 of 560 9.1 / 9.0 in a graph and 8.3 / 10.9 call by call).
 //
 // Long contexts among short ones: without splits there are helpers; with them, up to
 // WIDE_SPLITS for the contexts that have PART pairs for each (us, without / with: one of
@@ -851,7 +851,7 @@ __global__ __launch_bounds__(NW * 64, NB == 1 ? 3 : 2) void scaled_few_kernel(co
 struct Shape {
   int waves, base, splits, help;
 };
-constexpr long UNIT_BLOCKS = 256, TWO_BLOCKS = 512, SHORT = 6;
+constexpr long UNIT_BLOCKS = 256, TWO_BLOCKS = 512, SHORT = 4;
 constexpr long HELP_READS = 8192, WIDE_SPLITS = 16;
 
 // From which length of a sequence on a launch takes the longest first: blocks that all
