@@ -360,6 +360,31 @@ class TestDecode:
         near(got, c)
         assert torch.equal(got, decode(d))
 
+    @pytest.mark.gpu
+    @pytest.mark.parametrize("S", [12, 40, 70])
+    def test_replayed_with_other_lengths(self, S):
+        """A captured call whose long sequences are others at every replay."""
+        g = torch.Generator().manual_seed(S)
+        c = attention_case([8992] + [16] * (S - 1), [1] * S, 16, 8, 64, 47)
+        ids = c["table"][0, :562]
+        c["table"] = torch.stack([ids[torch.randperm(562, generator=g)] for _ in range(S)])
+        d = on(c, "cuda")
+        side = torch.cuda.Stream()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            decode(d)
+        torch.cuda.current_stream().wait_stream(side)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            got = decode(d)
+        for long in ([], [0], [S - 1, 3], [1, 2, 5, 6, 7, 8], list(range(S))):
+            c["ctx"] = torch.randint(0, 90, (S,), generator=g).int()
+            c["ctx"][long] = torch.randint(4000, 8993, (len(long),), generator=g).int()
+            d["ctx"].copy_(c["ctx"])
+            graph.replay()
+            near(got, c)
+            assert torch.equal(got, decode(d))
+
     @pytest.mark.parametrize("dev", devices())
     def test_extreme_scales(self, dev):
         """Pages from 2^-90 to 2^13 beside one another."""
