@@ -160,7 +160,11 @@ def reshape_and_cache(
     writes a page's first row begins the page anew under it; otherwise the page keeps
     the larger of its own and the new one, to which its other rows are rounded. Slots
     below 0 or behind the cache are left out; of a slot given twice the later row stays.
-    Infinities become the largest number of the page."""
+    Infinities become the largest number of the page.
+
+    Any scale byte may stand in a cache that is given: 0 is 2^-127, as for the type. 255 is
+    no number: attention reads the page's values as none, and a write that keeps its other
+    rows takes them for zeros."""
     if k.is_cuda and (k_scale is not None or v_scale is not None):
         _native("reshape_and_cache").write_scaled_pages(
             k, v, k_cache, v_cache, *_both_scales(k_scale, v_scale), slot_mapping

@@ -119,14 +119,14 @@ __device__ __forceinline__ float half_sum(float x) {
   return __uint_as_float(r[0]) + __uint_as_float(r[1]);
 }
 
-// 2^e as the widening conversions take it, from e's E8M0 byte (0, 2^-127, as the least
-// normal number: a page that holds nothing)
+// 2^e as the widening conversions take it, from e's E8M0 byte. They read the bits of the
+// exponent alone: 0 is 2^-127 and 255 no number, which all that it multiplies becomes.
 __device__ __forceinline__ float page_scale(unsigned int e) {
-  return __uint_as_float(max(e, 1u) << 23);
+  return __uint_as_float(e << 23);
 }
 
 // four E4M3 bytes each of two pages, times the pages' powers of two, as bf16 (exact: 4
-// bits of 8)
+// bits of 8, but for what falls below bf16's least number, 2^-133, or past its largest)
 __device__ __forceinline__ bf16x8_t widen_pages(uint2 x, float first, float second) {
   uint4 o;
   o.x = __builtin_bit_cast(unsigned int, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(x.x, first, false));

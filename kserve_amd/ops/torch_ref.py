@@ -158,8 +158,10 @@ def check_scaled_pages(k_cache, v_cache, k_scale, v_scale) -> None:
 
 
 def scaled_pages(cache: torch.Tensor, scale: torch.Tensor) -> torch.Tensor:
-    """The values [pages, kv_heads, block, D] that a block-scaled cache holds, in fp32."""
-    return torch.ldexp(cache.float(), (scale.view(torch.uint8).int() - 127)[..., None, None])
+    """The values [pages, kv_heads, block, D] that a block-scaled cache holds, in fp32: a
+    scale byte of 255 is no number, and none of its page's values is one."""
+    e = scale.view(torch.uint8).int()[..., None, None]
+    return torch.ldexp(cache.float(), e - 127).masked_fill(e == 255, math.nan)
 
 
 def scaled_context(

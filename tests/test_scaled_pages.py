@@ -694,3 +694,57 @@ class TestRefusals:
         for x, s in [(k, slots[:1]), (k, slots.long()), (k, slots.cpu()), (k.float(), slots), (k[:, :1], slots)]:
             with pytest.raises(RuntimeError):
                 ops.reshape_and_cache(x, x, c["kc"], c["vc"], s, k_scale=c["ks"], v_scale=c["vs"])
+
+
+def kinds(c, chunk):
+    """A case's attention by decode, by few queries or by a chunk's kernel."""
+    return context(c) if chunk else decode(c)
+
+
+class TestScaleBytes:
+    """Every byte a scale may have, at the ends of E8M0's range too.
+
+    There bf16, in which pages are multiplied, has steps of 2^-133 below its normal
+    numbers: a value may be off by half of one, 2^-134, which is
+    - 2^-134 of the outputs (weights sum to 1), and once more where outputs are rounded;
+    - of scores the sum of |q| 2^-134 times the scale, which moves a weight by that factor
+      above and the denominator by it below."""
+
+    @pytest.mark.parametrize("dev", devices())
+    @pytest.mark.parametrize("least", [0, 1, 5])
+    @pytest.mark.parametrize("new", [1, 4, 40])
+    def test_least_scales(self, dev, new, least):
+        g = torch.Generator().manual_seed(least)
+        c = attention_case([50, 100], [min(new, 40), new], 8, 2, 128, 230)
+        for n in ("ks", "vs"):
+            e = least + torch.randint(0, 3, c[n].shape, generator=g)
+            c[n] = e.to(torch.uint8).view(E8M0)
+        # scores of a few units all the same
+        c["scale"] = 2.0 ** (110 - least)
+        got = kinds(on(c, dev), new > 1)
+        out, off, size = attention_oracle(c)
+        lost = 2.0**-134
+        moved = 2 * c["q"].double().abs().sum(-1, keepdim=True) * c["scale"] * lost
+        off = off + 2 * lost + moved * size + (2.0**-8 * size if new > 1 else 0)
+        # (the bound tells 2^-127 from 2^-126)
+        assert float((off / out.abs().amax(-1, keepdim=True)).max()) < 0.1
+        assert bool(((got.double().cpu() - out).abs() <= off).all())
+
+    @pytest.mark.parametrize("dev", devices())
+    @pytest.mark.parametrize("new", [1, 4, 40])
+    @pytest.mark.parametrize("which", ["ks", "vs"])
+    def test_no_number(self, dev, new, which):
+        """Byte 255: what sees the page is no number, nothing else is touched."""
+        c = attention_case([50, 100], [new, new], 8, 2, 64, 240)
+        page = int(c["table"][0, 0])
+        c["vc"].view(torch.uint8)[page, 1] = 56  # (one sign: as infinities they would add up)
+        c[which].view(torch.uint8)[page, 1] = 255
+        got = kinds(on(c, dev), new > 1).cpu()
+        # query heads 4 to 7 read KV head 1
+        assert bool(got[:new, 4:].isnan().all())
+        assert not got[:new, :4].isnan().any() and not got[new:].isnan().any()
+        c[which].view(torch.uint8)[page, 1] = 120
+        out, off, size = attention_oracle(c)
+        off = off + (2.0**-8 * size if new > 1 else 0)
+        near_by = (got.double() - out).abs() <= off
+        assert bool(near_by[:new, :4].all()) and bool(near_by[new:].all())
