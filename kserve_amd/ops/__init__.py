@@ -195,7 +195,8 @@ def paged_attention_decode(
     """One query token per sequence against its pages. With ``k_scale`` and ``v_scale``
     the pages are block-scaled (``reshape_and_cache``): heads of 64 or 128, groups of up
     to 8; a page id outside the cache is read as its nearest page, a context longer than
-    its table row as one that fills it."""
+    its table row as one that fills it; what lies behind the context or ahead of the window
+    may be anything."""
     if q.is_cuda and (k_scale is not None or v_scale is not None):
         if out is None:
             out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
@@ -258,7 +259,7 @@ def context_attention_varlen(
     to the whole per-seq context (bounded below by the sliding window when
     window > 0). With ``k_scale`` and ``v_scale`` the pages are block-scaled
     (``reshape_and_cache``): heads of 64 or 128; page ids and contexts are bounded as in
-    ``paged_attention_decode``."""
+    ``paged_attention_decode``, and what no query of a sequence sees may be anything."""
     if q.is_cuda and (k_scale is not None or v_scale is not None):
         out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
         _native("context_prefill").context_prefill_scaled(

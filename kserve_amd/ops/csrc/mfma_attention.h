@@ -302,10 +302,15 @@ __global__ __launch_bounds__(256, 2) void prefill_attention_kernel(
 
   // ---- staging: wave w brings rows 16 w .. 16 w + 15 of a tile (one page);
   // rows past the keys repeat the last one (their weights are 0, their values
-  // finite) ----
+  // finite), and over block-scaled pages those ahead of the window the first one: bytes
+  // and scales there may be no numbers ----
+  constexpr bool FROM_LOW = SRC == PAGES_FP8S && WIN;
   const int* bt = PAGED ? p.block_tables + (long)seq * p.max_nb : nullptr;
   const int lrow = lane / CPR, lchunk = lane % CPR;
-  auto group_of = [&](int t) { return min(t * KT + wave * 16, len - 1); };
+  auto group_of = [&](int t) {
+    const int g = t * KT + wave * 16;
+    return min(FROM_LOW ? max(g, lo) : g, len - 1);
+  };
   auto page_of = [&](int t) {
     return PAGED && SRC != PAGES_FP8S ? bt[group_of(t) >> 4] : 0;
   };
@@ -378,18 +383,22 @@ __global__ __launch_bounds__(256, 2) void prefill_attention_kernel(
     const int g0 = PAGED ? group_of(t) & ~15 : group_of(t);
     const char* kb = base_of(p.k, krs, g0, page);
     const char* vb = base_of(p.v, vrs, g0, page);
-    if (KEEP && (t + 1) * KT <= len)
+    auto row = [&](int r) {
+      const int x = min(r, len - 1 - g0);
+      return FROM_LOW ? max(x, lo - g0) : x;
+    };
+    if (KEEP && (t + 1) * KT <= len && (!FROM_LOW || t * KT >= lo))
       stage_rows(kb, vb, [&](int i) { return koff[i]; }, [&](int i) { return voff[i]; }, buf);
     else
       stage_rows(
           kb, vb,
           [&](int i) {
             const int r = i * RPI + lrow;
-            return (unsigned int)(min(r, len - 1 - g0) * krs + (lchunk ^ k_swz<D>(r)) * 8) * ES;
+            return (unsigned int)(row(r) * krs + (lchunk ^ k_swz<D>(r)) * 8) * ES;
           },
           [&](int i) {
             const int r = i * RPI + lrow;
-            return (unsigned int)(min(r, len - 1 - g0) * vrs + (lchunk ^ v_swz<D>(r)) * 8) * ES;
+            return (unsigned int)(row(r) * vrs + (lchunk ^ v_swz<D>(r)) * 8) * ES;
           },
           buf);
   };

@@ -227,7 +227,8 @@ def paged_attention_decode(
     k_scale: Optional[torch.Tensor] = None,  # [num_blocks, num_kv_heads] E8M0
     v_scale: Optional[torch.Tensor] = None,
 ) -> torch.Tensor:
-    if k_scale is not None or v_scale is not None:
+    scaled = k_scale is not None or v_scale is not None
+    if scaled:
         k_cache, v_cache, block_tables, context_lens = scaled_context(
             q, k_cache, v_cache, k_scale, v_scale, block_tables, context_lens, window
         )
@@ -247,6 +248,9 @@ def paged_attention_decode(
         vals = v_cache[blocks].permute(1, 0, 2, 3).reshape(num_kv_heads, -1, head_dim)[
             :, :ctx
         ]
+        if scaled and window > 0:  # what lies ahead of it may be no numbers
+            keys, vals = keys[:, -window:], vals[:, -window:]
+            ctx = min(ctx, window)
         qh = q[s].float()  # [H, D]
         scores = torch.einsum(
             "hd,htd->ht", qh, keys.float().repeat_interleave(group, dim=0)
@@ -336,11 +340,15 @@ def context_attention_varlen(
             :, :ctx
         ].float().repeat_interleave(group, dim=0)
         qs = q[a:b].float().transpose(0, 1)  # [H, n_new, D]
-        scores = torch.einsum("htd,hsd->hts", qs, keys) * scale
         # causal: new token i (absolute pos ctx - n_new + i) sees pos <= its own
         start = ctx - n_new
+        first = 0
+        if scaled and window > 0:  # what lies ahead of the first one's may be no numbers
+            first = min(max(start - window + 1, 0), ctx)
+            keys, vals = keys[:, first:], vals[:, first:]
+        scores = torch.einsum("htd,hsd->hts", qs, keys) * scale
         pos_q = torch.arange(start, ctx, device=q.device).unsqueeze(1)
-        pos_k = torch.arange(ctx, device=q.device).unsqueeze(0)
+        pos_k = torch.arange(first, ctx, device=q.device).unsqueeze(0)
         bad = pos_k > pos_q
         if window > 0:
             bad |= pos_k <= pos_q - window

@@ -748,3 +748,37 @@ class TestScaleBytes:
         off = off + (2.0**-8 * size if new > 1 else 0)
         near_by = (got.double() - out).abs() <= off
         assert bool(near_by[:new, :4].all()) and bool(near_by[new:].all())
+
+
+class TestAheadOfTheWindow:
+    @pytest.mark.parametrize("dev", devices())
+    @pytest.mark.parametrize("D", [64, 128])
+    @pytest.mark.parametrize(
+        "window, new",
+        [(1, 1), (20, 1), (48, 1), (3, 5), (40, 5), (1, 40), (20, 40), (65, 40), (100, 150), (90, 77)],
+    )
+    def test_may_be_anything(self, dev, D, window, new):
+        """Keys that no query of their sequence sees, in whole pages and in part of one: bytes
+        and scales that are no numbers, pages that are not the sequence's."""
+        lens = [max(new, 30), 300, 173]
+        c = attention_case(lens, [new] * 3, 8, 2, D, 250, window)
+        near(kinds(on(c, dev), new > 1), c, new > 1)
+        for i, n in enumerate(lens):
+            low = max(n - new - window + 1, 0)
+            pages, rows = c["table"][i, : low // PAGE].long(), low % PAGE
+            for scale, cache in (("ks", "kc"), ("vs", "vc")):
+                c[scale].view(torch.uint8)[pages] = 255
+                c[cache].view(torch.uint8)[c["table"][i, low // PAGE], :, :rows] = 0x7F
+            c["table"][i, : low // PAGE // 2] = -7
+        # (page 0, where those now point, is nobody's)
+        c["ks"].view(torch.uint8)[0] = c["vs"].view(torch.uint8)[0] = 255
+        d = dict(c, table=c["table"].clamp(min=0))
+        for n in ("kc", "vc"):  # the oracle's: numbers, which it gives no weight
+            raw = c[n].view(torch.uint8).clone()
+            raw[raw % 128 == 127] = 0
+            d[n] = raw.view(E4M3)
+        for n in ("ks", "vs"):
+            raw = c[n].view(torch.uint8).clone()
+            raw[raw == 255] = 118
+            d[n] = raw.view(E8M0)
+        near(kinds(on(c, dev), new > 1), d, new > 1)
