@@ -842,7 +842,12 @@ __global__ __launch_bounds__(NW * 64, NB == 1 ? 3 : 2) void scaled_few_kernel(co
 // of 131071 under groups of eight 83 / 53 / 53 with 16, 32 and 64, of 7000 18.0 / 15.0 / 16.0
 // with 8, 16 and 32), unless eight waves take a table in SHORT pairs each, which spares the
 // launch that merges (eight waves / splits: 1 of 1500 13.7 / 9.3, 8 of 1500 13.9 / 10.7, 20
-// of 1000 12.0 / 15.1; 1 of 560 9.1 / 9.0 in a graph and 8.3 / 10.9 call by call).
+// of 1000 12.0 / 15.1; 1 of 560 9.1 / 9.0 in a graph and 8.3 / 10.9 call by call). In wider
+// tables it is a window that is short: in SHORT pairs from WINDOW_BLOCKS on, in half as many
+// below, where a captured launch that merges costs less than the pairs (eight waves / splits
+// in a graph, and call by call: 1 behind 255 7.2 / 7.7, 7.2 / 11.1, 8 behind 384 8.3 / 8.1, 8.3
+// / 10.8, behind 1000 10.8 / 9.1, 10.7 / 10.9, 12 behind 1000 11.0 / 12.3, 16 behind 255 7.4 /
+// 9.2, 20 behind 1000 11.5 / 14.6).
 //
 // Long contexts among short ones: without splits there are helpers; with them, up to
 // WIDE_SPLITS for the contexts that have PART pairs for each (us, without / with: one of
@@ -851,7 +856,7 @@ __global__ __launch_bounds__(NW * 64, NB == 1 ? 3 : 2) void scaled_few_kernel(co
 struct Shape {
   int waves, base, splits, help;
 };
-constexpr long UNIT_BLOCKS = 256, TWO_BLOCKS = 512, SHORT = 4;
+constexpr long UNIT_BLOCKS = 256, TWO_BLOCKS = 512, SHORT = 4, WINDOW_BLOCKS = 96;
 constexpr long HELP_READS = 8192, WIDE_SPLITS = 16;
 
 // From which length of a sequence on a launch takes the longest first: blocks that all
@@ -867,10 +872,13 @@ Shape decode_shape(long seqs, long kv_heads, long max_blocks, int window) {
   const long reads = window > 0 && window < max_blocks * PAGE ? window : max_blocks * PAGE;
   const int help = seqs > 0 && seqs <= LAST && reads >= HELP_READS ? HELP : 0;
   if (blocks <= 0 || blocks >= TWO_BLOCKS) return {4, 1, 1, help};
-  const long pairs = (max_blocks + 1) / 2;
+  // pages that a query sees: of a window's first and last key, and between them
+  const long seen = window > 0 ? (window + PAGE - 2L) / PAGE + 1 : max_blocks;
+  const long pairs = ((seen < max_blocks ? seen : max_blocks) + 1) / 2;
   long splits = (UNIT_BLOCKS + blocks / 2) / blocks;
   if (splits <= 1) return {8, 1, 1, help};
-  if (pairs <= 8 * SHORT) return {8, 1, 1, 0};
+  const bool narrow = max_blocks <= 2 * 8 * SHORT;
+  if (narrow || pairs <= 8 * (blocks >= WINDOW_BLOCKS ? SHORT : SHORT / 2)) return {8, 1, 1, 0};
   const long most = (pairs + 3) / 4;  // a pair for every wave
   splits = splits < most ? splits : most;
   const long whole = reads / (2 * PAGE) / PART;

@@ -427,3 +427,22 @@ def test_blocks_of_gated_activations(native, d):
         got = blocks(rows, d)
         want = rows * -(-d // 2048) if by_rows else -(-rows * (d // 8) // 256)
         assert got == min(want, (1 << 24) - 1) and got * 256 < 1 << 32
+
+
+@pytest.mark.parametrize("seqs", [1, 4, 11, 12, 16, 24, 32, 100])
+@pytest.mark.parametrize("window", [1, 2, 17, 18, 255, 480, 512, 1000, 1009, 4096, 9000])
+def test_decode_behind_a_window(native, seqs, window):
+    """Block-scaled decode behind a window: however wide the tables, the launch is made for
+    the pages that the window can reach."""
+    shape = native.ks_scaled_decode_shape
+    # (keys i + 1 .. i + window of the worst i)
+    reach = max((i + window) // 16 - (i + 1) // 16 + 1 for i in range(16))
+    pairs = (reach + 1) // 2
+    want = shape(seqs, 8, max(reach, 65), window)
+    for wide in (max(reach, 65) + 1, 600, 8192, 1 << 20):
+        assert shape(seqs, 8, max(wide, reach), window) == want
+    waves, splits = want & 255, want >> 8 & 0xFFFF
+    # a pair for every wave of every split, or contexts that have 128 for each
+    assert splits <= max(-(-pairs // 4), pairs // 128, 1)
+    if seqs < 24 and pairs <= (32 if seqs >= 12 else 16):
+        assert (waves, splits) == (8, 1)

@@ -782,3 +782,17 @@ class TestAheadOfTheWindow:
             raw[raw == 255] = 118
             d[n] = raw.view(E8M0)
         near(kinds(on(c, dev), new > 1), d, new > 1)
+
+
+class TestWindowsInWideTables:
+    @pytest.mark.gpu
+    @pytest.mark.parametrize("S", [1, 5, 13, 25, 70])
+    @pytest.mark.parametrize("window", [1, 255, 500, 1000, 2500])
+    def test_few_sequences(self, S, window):
+        """In one part and in several, by what the window reaches."""
+        g = torch.Generator().manual_seed(S)
+        lens = torch.randint(1, 3000, (S,), generator=g)
+        lens[0], lens[-1] = window + 17, 2999
+        c = attention_case(lens.tolist(), [1] * S, 8, 8, 64, 270, window)
+        c["table"] = torch.nn.functional.pad(c["table"], (0, 900))
+        near(decode(on(c, "cuda")), c)
