@@ -309,6 +309,12 @@ void check_scaled_attention(const at::Tensor& out, const at::Tensor& q,
               "scaled pages: sizes out of range");
 }
 
+// A window no shorter than the tables hides nothing, and is none: sums of positions and
+// windows stay within 32 bits.
+int scaled_window(int64_t window, const at::Tensor& tables) {
+  return window < tables.size(1) * 16 ? (int)window : 0;
+}
+
 void paged_attention_decode_scaled(at::Tensor& out, at::Tensor& q, at::Tensor& k_cache,
                                    at::Tensor& v_cache, at::Tensor& k_scale,
                                    at::Tensor& v_scale, at::Tensor& block_tables,
@@ -320,7 +326,8 @@ void paged_attention_decode_scaled(at::Tensor& out, at::Tensor& q, at::Tensor& k
   TORCH_CHECK(H / Hkv <= 8, "scaled pages: groups of up to 8 heads in decode");
   const c10::DeviceGuard guard(q.device());
   const int max_blocks = block_tables.size(1);
-  const int shape = ks_scaled_decode_shape(S, Hkv, max_blocks, (int)window);
+  const int win = scaled_window(window, block_tables);
+  const int shape = ks_scaled_decode_shape(S, Hkv, max_blocks, win);
   const int n_splits = shape >> 8 & 0xffff, help = shape >> 24;
   at::Tensor part_out, part_ml;
   void *po = nullptr, *pml = nullptr;
@@ -336,7 +343,7 @@ void paged_attention_decode_scaled(at::Tensor& out, at::Tensor& q, at::Tensor& k
                 out.data_ptr(), q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(),
                 k_scale.data_ptr(), v_scale.data_ptr(), block_tables.data_ptr(),
                 context_lens.data_ptr(), (float)scale, S, H, Hkv, D, max_blocks,
-                (int)k_cache.size(0), (long)q.stride(0), shape, po, pml, (int)window,
+                (int)k_cache.size(0), (long)q.stride(0), shape, po, pml, win,
                 current_stream()),
             "paged_attention_decode");
 }
@@ -426,9 +433,10 @@ void context_prefill_scaled(at::Tensor& out, at::Tensor& q, at::Tensor& k_cache,
   // (no sequence has more queries than there are)
   const int longest = (int)std::min<int64_t>(std::max<int64_t>(max_q_len, 0), q.size(0));
   const long rows = (long)q.size(0) * Hq;
+  const int win = scaled_window(window, block_tables);
   const int n_splits =
       ks_context_scaled_splits((int)seqs, rows, longest, Hq, Hkv, (int)block_tables.size(1),
-                               (int)window);
+                               win);
   TORCH_CHECK(seqs * n_splits < 65536, "scaled pages: sizes out of range");
   at::Tensor part_out, part_ml;
   void *po = nullptr, *pml = nullptr;
@@ -444,7 +452,7 @@ void context_prefill_scaled(at::Tensor& out, at::Tensor& q, at::Tensor& k_cache,
                 k_scale.data_ptr(), v_scale.data_ptr(), block_tables.data_ptr(),
                 ctx_lens.data_ptr(), cu_seqlens_q.data_ptr(), (int)seqs, longest, Hq, Hkv, D,
                 (int)block_tables.size(1), (int)k_cache.size(0), (float)scale,
-                (long)q.stride(0), (int)window, rows, n_splits, po, pml, current_stream()),
+                (long)q.stride(0), win, rows, n_splits, po, pml, current_stream()),
             "context_attention_varlen");
 }
 

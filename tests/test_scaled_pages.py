@@ -796,3 +796,18 @@ class TestWindowsInWideTables:
         c = attention_case(lens.tolist(), [1] * S, 8, 8, 64, 270, window)
         c["table"] = torch.nn.functional.pad(c["table"], (0, 900))
         near(decode(on(c, "cuda")), c)
+
+
+class TestWindowsPastTheTables:
+    @pytest.mark.parametrize("dev", devices())
+    @pytest.mark.parametrize("new", [1, 5, 70])
+    @pytest.mark.parametrize("window", [2**31 - 1, 2**31 - 60, 1000])
+    def test_hide_nothing(self, dev, new, window):
+        """The results are those without a window; of contexts shorter than their queries too,
+        whose first ones stand ahead of position 0."""
+        c = attention_case([70, 300, 90], [new] * 3, 8, 2, 64, 260)
+        c["ctx"][2] = max(new - 4, 1)
+        d = on(c, dev)
+        got = kinds(dict(d, window=window), new > 1)
+        near(got, c, new > 1)
+        assert torch.equal(got, kinds(d, new > 1))
