@@ -317,6 +317,14 @@ class ModelRunner:
         return comm.get_state().tp_size
 
     # -- input prep -----------------------------------------------------------
+    # Tokens of a single prompt up to which its positions and slots are formed on the
+    # host. The kernel that forms them is 3 to 4 us of the GPU's, ahead of the model's first,
+    # and spares the host time that grows with the tokens (four llama layers 4096 wide, us,
+    # host / kernel among passes, and where the GPU is waited for: 16 tokens 443 / 448, 574 /
+    # 572, 77 510 / 513, 637 / 633, 128 575 / 578, 700 / 695, 200 699 / 702, 836 / 828, 400
+    # 1142 / 1148, 1322 / 1300; four prompts of 77 1008 / 1012, 1189 / 1172).
+    HOST_TOKENS = 128
+
     def prepare_prefill(
         self, batch: ScheduledBatch, block_manager: BlockManager, logit_rows=None
     ):
@@ -366,11 +374,16 @@ class ModelRunner:
     def _paged_batch(self, requests, widths, block_manager, arrays, tables: bool = True):
         """(the arrays on the device, what attention is told of the batch): the next
         ``widths`` tokens of each request. Page lists and lengths go up with the arrays;
-        positions, slots and page tables (empty ones unless asked for) are made there."""
+        positions, slots and page tables (empty ones unless asked for) are made there;
+        those of a short prompt without tables here."""
         import numpy as np
 
         bs = self.config.cache.block_size
         computed = [r.num_computed_tokens for r in requests]
+        if not tables and len(widths) == 1 and widths[0] <= self.HOST_TOKENS:
+            arrays = [*arrays, *self._prompt_rows(requests[0], widths[0], block_manager)]
+            *out, positions, slots, cu, seqs = self._to_device(arrays)
+            return out, ops.PagedBatch(positions, slots, cu, None, None, seqs)
         # page ids, where each request's begin, computed and new lengths: one array
         ints, starts, widest = [], [0], 0
         for r, c, n in zip(requests, computed, widths):
@@ -392,6 +405,22 @@ class ModelRunner:
         )
         return out, made
 
+    def _prompt_rows(self, request, n, block_manager):
+        """Positions, slots, cu_seqlens and request of the next ``n`` tokens."""
+        import numpy as np
+
+        bs, start = self.config.cache.block_size, request.num_computed_tokens
+        first, used = start // bs, -(-(start + n) // bs)
+        table = block_manager.get_block_table(request)
+        if len(table) < used:
+            raise IndexError(f"request {request.request_id}: {len(table)} pages of {used}")
+        rows = np.arange(bs) + np.array(table[first:used], dtype=np.int64)[:, None] * bs
+        at = start - first * bs
+        return (
+            np.arange(start, start + n), rows.reshape(-1)[at : at + n].astype(np.int32),
+            np.array([0, n], dtype=np.int32), np.zeros(n, dtype=np.int32),
+        )
+
     def _to_device(self, arrays) -> List[torch.Tensor]:
         """The arrays on the device. A GPU gets them in one copy out of pinned
         memory, which nothing waits for: with copies of lists among them the host
@@ -409,10 +438,13 @@ class ModelRunner:
         for a, at in zip(arrays, starts):
             rows[at : at + a.nbytes] = a.reshape(-1).view("uint8")
         block = staged.to(self.device, non_blocking=True)
-        return [
-            block[at : at + a.nbytes].view(_TORCH_INTS[a.dtype.itemsize]).view(a.shape)
-            for a, at in zip(arrays, starts)
-        ]
+        views = {n: block.view(t) for n, t in _TORCH_INTS.items()}
+        out = []
+        for a, at in zip(arrays, starts):
+            n = a.itemsize
+            t = views[n][at // n : at // n + a.size]
+            out.append(t if a.ndim == 1 else t.view(a.shape))
+        return out
 
     def _ensure_decode_buffers(self, n: int, max_blocks: int):
         """Pinned staging rows for a decode batch (read by one kernel) as

@@ -313,3 +313,54 @@ class TestRunnerTables:
         _, pos, meta, sel = r.prepare_prefill(batch, manager)
         assert pos.tolist() == [0, 1, 2, 0, 1, 0] and sel.tolist() == [2, 4, 5]
         assert meta.block_tables is None and meta.context_lens is None
+
+
+class TestShortPrompts:
+    @pytest.mark.parametrize("dev", devices())
+    @pytest.mark.parametrize("n", [0, 1, 16, 77, 128, 129])
+    def test_one_prompt(self, dev, n, monkeypatch):
+        """A short prompt's positions and slots go up with its tokens, and nothing is launched
+        for them."""
+        e = engine("auto", dev)
+        r, bs = e.runner, e.config.cache.block_size
+        manager = BlockManager(96, bs)
+        q = Request(request_id="0", prompt_token_ids=list(range(200)),
+                    sampling_params=SamplingParams(max_tokens=4))
+        manager.allocate(q, max(n, 1))
+        calls = []
+        build = ops.build_paged_batch
+        monkeypatch.setattr(ops, "build_paged_batch", lambda *a: calls.append(1) or build(*a))
+        batch = ScheduledBatch(is_prefill=True, requests=[q], num_scheduled_tokens=[n])
+        ids, pos, meta, sel = r.prepare_prefill(batch, manager)
+        assert len(calls) == (1 if n > 128 else 0)
+        table = manager.get_block_table(q)
+        assert ids.tolist() == pos.tolist() == list(range(n))
+        assert ids.dtype == pos.dtype == sel.dtype == torch.int64
+        assert meta.slot_mapping.tolist() == [table[p // bs] * bs + p % bs for p in range(n)]
+        assert meta.cu_seqlens.tolist() == [0, n] and sel.tolist() == [n - 1]
+        assert meta.slot_mapping.dtype == meta.cu_seqlens.dtype == torch.int32
+        assert meta.block_tables is None and meta.context_lens is None
+        assert {t.device.type for t in (ids, pos, sel, meta.slot_mapping, meta.cu_seqlens)} == {dev}
+        if n == 77:
+            batch = ScheduledBatch(is_prefill=True, requests=[q], num_scheduled_tokens=[120])
+            with pytest.raises(IndexError):  # more than its pages hold
+                r.prepare_prefill(batch, manager)
+
+    def test_resumed_prompts_have_tables(self):
+        """What was computed before is attended to by its pages, however few the tokens."""
+        e = engine("auto")
+        r, bs = e.runner, e.config.cache.block_size
+        manager = BlockManager(96, bs)
+        q = Request(request_id="0", prompt_token_ids=list(range(60)),
+                    sampling_params=SamplingParams(max_tokens=4))
+        manager.allocate(q, 60)
+        q.num_computed_tokens = 21
+        batch = ScheduledBatch(is_prefill=True, requests=[q], num_scheduled_tokens=[7])
+        ids, pos, meta, sel = r.prepare_prefill(batch, manager)
+        table = manager.get_block_table(q)
+        assert pos.tolist() == list(range(21, 28)) and meta.context_lens.tolist() == [28]
+        assert meta.block_tables.tolist() == [table[: -(-28 // bs)]]
+        r.kv_caches = []  # (without pages there is nothing to attend to)
+        ids, pos, meta, sel = r.prepare_prefill(batch, manager)
+        assert pos.tolist() == ids.tolist() == list(range(21, 28)) and meta.block_tables is None
+        assert meta.slot_mapping.tolist() == [table[p // bs] * bs + p % bs for p in range(21, 28)]
