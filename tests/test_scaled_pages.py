@@ -811,3 +811,65 @@ class TestWindowsPastTheTables:
         got = kinds(dict(d, window=window), new > 1)
         near(got, c, new > 1)
         assert torch.equal(got, kinds(d, new > 1))
+
+
+class TestLongParts:
+    """Parts of more keys than a wave holds page ids and scales for (4096: 64 tiles of the
+    chunk kernel, 32 pairs of pages of each of four waves), which it fetches anew."""
+
+    def parts(self, c):
+        """Key parts that such a call is cut into."""
+        import ctypes
+
+        rule = ctypes.CDLL(ops._C.__file__).ks_context_scaled_splits
+        rule.argtypes = [ctypes.c_int, ctypes.c_long] + [ctypes.c_int] * 5
+        S, longest = len(c["ctx"]), int((c["cu"][1:] - c["cu"][:-1]).max())
+        H, kv = c["q"].shape[1], c["kc"].shape[1]
+        return rule(S, c["q"].shape[0] * H, longest, H, kv, c["table"].shape[1], c["window"])
+
+    def check(self, c, heads):
+        """By some KV heads (and one query head of each)."""
+        got = context(on(c, "cuda"))
+        G = c["q"].shape[1] // c["kc"].shape[1]
+        some = torch.tensor(heads)
+        few = dict(c, q=c["q"][:, some * G])
+        for n in ("kc", "vc", "ks", "vs"):
+            few[n] = c[n].view(torch.uint8)[:, some].contiguous().view(c[n].dtype)
+        near(got[:, some * G], few, True)
+
+    @pytest.mark.gpu
+    @pytest.mark.parametrize("D, kv, window", [(64, 128, 0), (64, 128, 5003), (128, 128, 8200)])
+    def test_chunks_in_one_part(self, D, kv, window):
+        c = attention_case([9001], [512], kv, kv, D, 280, window)
+        assert self.parts(c) == 1
+        self.check(c, [0, 77, 127])
+
+    @pytest.mark.gpu
+    @pytest.mark.parametrize("window", [0, 139000])
+    def test_chunks_in_several(self, window):
+        c = attention_case([140003], [70], 2, 1, 64, 290, window)
+        c["table"] = c["table"][:, :8751].contiguous()
+        assert self.parts(c) * 4096 < min(140003, window or 140003)
+        self.check(c, [0])
+
+    @pytest.mark.gpu
+    @pytest.mark.parametrize("D", [64, 128])
+    @pytest.mark.parametrize("window", [0, 6005])
+    @pytest.mark.parametrize("most", [4, 20, 40])
+    def test_few_queries_in_one_part(self, D, window, most):
+        g = torch.Generator().manual_seed(most)
+        new = torch.randint(1, most + 1, (32,), generator=g)
+        lens = new + torch.randint(0, 60, (32,), generator=g)
+        lens[3], lens[20], lens[31], new[20] = 9001, 4130, 12345, most
+        c = attention_case(lens.tolist(), new.tolist(), 8, 8, D, 300, window)
+        assert self.parts(c) == 1
+        self.check(c, [0, 5])
+
+    @pytest.mark.gpu
+    @pytest.mark.parametrize("window", [0, 18001])
+    def test_few_queries_in_several(self, window):
+        lens = [40 + i for i in range(16)]
+        lens[2] = 20007
+        c = attention_case(lens, [3] * 16, 16, 8, 64, 310, window)
+        assert self.parts(c) == 2
+        self.check(c, [0, 7])
