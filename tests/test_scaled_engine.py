@@ -364,3 +364,123 @@ class TestShortPrompts:
         ids, pos, meta, sel = r.prepare_prefill(batch, manager)
         assert pos.tolist() == ids.tolist() == list(range(21, 28)) and meta.block_tables is None
         assert meta.slot_mapping.tolist() == [table[p // bs] * bs + p % bs for p in range(21, 28)]
+
+
+class Watch:
+    """Every write to a model's cache and every attention over it, layer by layer, against
+    what the layer's own four tensors hold: K under K's scales, V under V's."""
+
+    def __init__(self, runner, monkeypatch):
+        self.caches = runner.kv_caches
+        self.writes = self.reads = 0
+        self.real = {n: getattr(ops, n) for n in (
+            "reshape_and_cache", "paged_attention_decode", "context_attention_varlen")}
+        monkeypatch.setattr(ops, "reshape_and_cache", self.write)
+        monkeypatch.setattr(ops, "paged_attention_decode", self.decode)
+        monkeypatch.setattr(ops, "context_attention_varlen", self.context)
+
+    def write(self, k, v, k_cache, v_cache, slots, *more, **named):
+        self.real["reshape_and_cache"](k, v, k_cache, v_cache, slots, *more, **named)
+        kc, vc, ks, vs = self.caches[self.writes % len(self.caches)]
+        self.writes += 1
+        at = slots[: k.shape[0]].cpu().long()
+        assert bool((at >= 0).all())
+        for rows, cache, scale in ((k, kc, ks), (v, vc, vs)):
+            got = held(cache, scale)[at // PAGE, :, at % PAGE]
+            step = torch.exp2(scale.view(torch.uint8).cpu().double() - 127)[at // PAGE]
+            # half a step of E4M3, 2^-10 of the scale below its normal numbers
+            off = 2.0**-4 * rows.cpu().double().abs() + 2.0**-10 * step[..., None]
+            assert bool(((got - rows.cpu().double()).abs() <= off).all())
+
+    def near(self, got, q, tables, ctx, cu, scale, window, chunk):
+        kc, vc, ks, vs = self.caches[self.reads % len(self.caches)]
+        self.reads += 1
+        near(got, dict(
+            q=q.cpu(), kc=kc, vc=vc, ks=ks, vs=vs, table=tables.cpu(), ctx=ctx.cpu(), cu=cu.cpu(),
+            scale=scale, window=window), chunk)
+        return got
+
+    def decode(self, q, k_cache, v_cache, tables, ctx, scale, window=0, **named):
+        got = self.real["paged_attention_decode"](
+            q, k_cache, v_cache, tables, ctx, scale, window=window, **named)
+        cu = torch.arange(q.shape[0] + 1, dtype=torch.int32)
+        return self.near(got, q, tables, ctx, cu, scale, window, False)
+
+    def context(self, q, k_cache, v_cache, tables, cu, ctx, longest, scale, window=0, **named):
+        got = self.real["context_attention_varlen"](
+            q, k_cache, v_cache, tables, cu, ctx, longest, scale, window=window, **named)
+        return self.near(got, q, tables, ctx, cu, scale, window, True)
+
+
+class NoAdapter:
+    """Adapters that add nothing: the layers take the path that applies them."""
+
+    def apply(self, *a):
+        pass
+
+    def delta_for(self, *a):
+        return None
+
+
+class TestEachStep:
+    @pytest.mark.parametrize("dev", devices())
+    @pytest.mark.parametrize("window, adapters", [(0, False), (24, False), (0, True)])
+    def test_reads_what_its_caches_hold(self, dev, window, adapters, monkeypatch):
+        """Prompts, chunks behind them, tokens one by one and drafts under verification over a
+        model whose values are far larger than its keys: every attention is that of K's bytes
+        under K's scales and V's under V's."""
+        e = engine("fp8_scaled", dev, block_size=16)
+        r = e.runner
+        for i, layer in enumerate(r.model.layers):
+            w = layer.self_attn.qkv_proj.weight
+            w[-128:] *= 64.0 * 2**i  # 2 KV heads of 64
+            layer.self_attn.sliding_window = window
+        manager = BlockManager(96, 16)
+        g = torch.Generator().manual_seed(8)
+        reqs = []
+        for i in range(3):
+            q = Request(request_id=str(i), prompt_token_ids=torch.randint(
+                0, 512, (200,), generator=g).tolist(), sampling_params=SamplingParams(max_tokens=4))
+            manager.allocate(q, 120)
+            reqs.append(q)
+        w = Watch(r, monkeypatch)
+
+        def batch(new):
+            return ScheduledBatch(is_prefill=max(new) > 1, requests=reqs, num_scheduled_tokens=new)
+
+        def done(new):
+            for q, n in zip(reqs, new):
+                q.num_computed_tokens += n
+
+        def prefill(new):
+            ids, pos, meta, sel = r.prepare_prefill(batch(new), manager)
+            if adapters:
+                meta.lora = NoAdapter()
+            with torch.no_grad():
+                out = r.model(ids, pos, r.kv_caches, meta)
+            assert out.shape[0] == sum(new) and bool(out.isfinite().all())
+            done(new)
+
+        prefill([37, 5, 16])
+        assert (w.writes, w.reads) == (2, 0)
+        prefill([11, 40, 1])
+        assert (w.writes, w.reads) == (4, 2)
+        for _ in range(2):
+            if adapters:
+                ids, pos, meta = r.prepare_decode(batch([1] * 3), manager)
+                meta.lora = NoAdapter()
+                with torch.no_grad():
+                    logits = r.model(ids, pos, r.kv_caches, meta)
+            else:
+                logits = r.execute_decode(batch([1] * 3), manager)
+            assert logits.shape[0] == 3 and bool(logits.isfinite().all())
+            done([1] * 3)
+        assert (w.writes, w.reads) == (8, 6)
+        logits, cu = r.execute_verify(batch([1] * 3), [[5, 6, 7], [], [9] * 7], manager)
+        assert cu == [0, 4, 5, 13] and logits.shape[0] == 13 and bool(logits.isfinite().all())
+        # two drafts of the first are taken, none of the last: the next rows go over the others'
+        done([3, 1, 1])
+        logits, cu = r.execute_verify(batch([1] * 3), [[8], [5, 2], []], manager)
+        assert (w.writes, w.reads) == (12, 10)
+        top = [[int(s.view(torch.uint8).max()) for s in layer[2:]] for layer in r.kv_caches]
+        assert all(v > k + 3 for k, v in top)  # (scales that are not to be told apart prove nothing)
