@@ -194,7 +194,8 @@ class ModelRunner:
             self._allocate_layout(num_blocks)
             return
         m = self.config.model
-        kv_heads_local = max(1, m.num_kv_heads // max(1, self._tp_size()))
+        tp = max(1, self._tp_size())
+        kv_heads_local = max(1, m.num_kv_heads // tp)
         shape = (
             num_blocks,
             kv_heads_local,
@@ -205,7 +206,7 @@ class ModelRunner:
         dtype = cache.cache_torch_dtype(self.model.dtype)
         if cache.scaled and self.is_cuda and (
             cache.block_size != 16 or m.head_dim not in (64, 128)
-            or m.num_heads > 8 * m.num_kv_heads
+            or m.num_heads // tp > 8 * kv_heads_local
         ):
             raise ValueError(
                 "kv_cache_dtype fp8_scaled: pages of 16 tokens, heads of 64 or 128 and "

@@ -484,3 +484,25 @@ class TestEachStep:
         assert (w.writes, w.reads) == (12, 10)
         top = [[int(s.view(torch.uint8).max()) for s in layer[2:]] for layer in r.kv_caches]
         assert all(v > k + 3 for k, v in top)  # (scales that are not to be told apart prove nothing)
+
+
+class TestSplitHeads:
+    @pytest.mark.parametrize(
+        "heads, kv, tp, taken",
+        [(64, 4, 8, True), (16, 1, 2, True), (64, 8, 1, True), (64, 4, 1, False), (32, 1, 2, False),
+         (72, 8, 8, False)],
+    )
+    def test_groups_are_a_ranks_own(self, heads, kv, tp, taken, monkeypatch):
+        """KV heads that are fewer than the ranks stand on several of them, with fewer query
+        heads each."""
+        r = engine("auto").runner
+        r.config.cache = CacheConfig(block_size=16, num_gpu_blocks=16, kv_cache_dtype="fp8_scaled")
+        r.config.model.num_heads, r.config.model.num_kv_heads = heads, kv
+        r.is_cuda = True  # (the kernels' limits; the pages stay on the host)
+        monkeypatch.setattr(r, "_tp_size", lambda: tp)
+        if taken:
+            r.allocate_kv_cache(16)
+            assert r.kv_caches[0][0].shape == (16, max(1, kv // tp), 16, 64)
+        else:
+            with pytest.raises(ValueError):
+                r.allocate_kv_cache(16)
