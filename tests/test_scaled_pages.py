@@ -873,3 +873,39 @@ class TestLongParts:
         c = attention_case(lens, [3] * 16, 16, 8, 64, 310, window)
         assert self.parts(c) == 2
         self.check(c, [0, 7])
+
+
+class TestLongWrites:
+    @pytest.mark.gpu
+    @pytest.mark.parametrize(
+        "T, kv, D, order",
+        [(2048, 9, 64, "runs"), (2049, 9, 64, "runs"), (5000, 8, 128, "any"), (8191, 4, 128, "runs"),
+         (9001, 9, 64, "twice"), (70001, 5, 64, "runs"), (66000, 1, 64, "any")],
+    )
+    def test_is_the_plain_form(self, T, kv, D, order):
+        """Prompts of more tokens than a block has, in several blocks to a page, whose slots
+        stand in runs, in any order, and twice; of a slot map at an odd address too."""
+        g = torch.Generator().manual_seed(T)
+        pages = T // PAGE + 40
+        kc, ks = make_cache(pages, kv, D, 16)
+        x = (torch.randn((T, 2 * kv, D), generator=g) * torch.exp(torch.randn((T, 1, 1), generator=g)))
+        x = x.to(torch.bfloat16)
+        if order == "runs":  # one sequence, from inside a page on
+            ids = torch.randperm(pages, generator=g)
+            at = torch.arange(T) + 5
+            slots = ids[at // PAGE] * PAGE + at % PAGE
+        elif order == "any":
+            slots = torch.randperm(pages * PAGE, generator=g)[:T]
+        else:
+            slots = torch.randint(-5, pages * PAGE + 5, (T,), generator=g)
+        slots = slots.int()
+        outs = []
+        for dev, skip in (("cpu", 0), ("cuda", 0), ("cuda", 1)):
+            c = [t.view(torch.uint8).to(dev).clone().view(t.dtype) for t in (kc, kc, ks, ks)]
+            sl = torch.cat([slots[:skip], slots]).to(dev)[skip:]
+            y = x.to(dev)
+            ops.reshape_and_cache(y[:, :kv], y[:, kv:], c[0], c[1], sl, k_scale=c[2], v_scale=c[3])
+            outs.append([t.view(torch.uint8).cpu() for t in c])
+        for got in outs[1:]:
+            for a, b in zip(got, outs[0]):
+                assert torch.equal(a, b)
