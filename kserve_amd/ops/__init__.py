@@ -157,8 +157,10 @@ def reshape_and_cache(
     With ``k_scale`` and ``v_scale`` (float8_e8m0fnu [pages, kv_heads]) the cache is
     float8_e4m3fn under one power of two per page of 16 tokens and KV head. New rows ask
     for the least that brings their largest finite value to 448 or below. A call that
-    writes a page's first row begins the page anew under it; otherwise the page keeps
-    the larger of its own and the new one, to which its other rows are rounded. Slots
+    writes a page's first row begins the page anew under it, and the rows that the call
+    does not write hold nothing from then on; otherwise the page keeps the larger of its
+    own and the new one, to which its other rows are rounded (so what a row that is
+    written over later, a draft's say, asked for stays with the page). Slots
     below 0 or behind the cache are left out; of a slot given twice the later row stays.
     Infinities become the largest number of the page.
 

@@ -97,10 +97,12 @@ __global__ void reshape_and_cache_fp8_kernel(
 // conversions, two numbers at a time. Of a page with one new row (a decode step's) it takes
 // four heads of 128 at once.
 //
-// Measured (8 KV heads of 128, us, on the GPU; K and V are read and written once at 4.9 TB/s
-// in brackets): 1 token 4.0, 256 tokens of as many sequences 4.7 (0.3), 1536 6.0 (2.0), 8
-// prompts of 1000 16.2 (10.3), 16 of 1000 26.0 (20.2). A few tokens are two memory accesses,
-// a barrier and one more; prompts are bound by how few pages they are (500, 16 waves each).
+// Measured (8 KV heads of 128, us, the kernel's trace; K and V are read and written once at
+// 4.9 TB/s in brackets): 1 token 2.4, 256 tokens of as many sequences 4.6 (0.3), 1536 6.2
+// (2.0), 8 prompts of 1000 16.5 (10.3), 16 of 1000 26.7 (20.2), 32 of 1024 62 (41), 64 of 1024
+// 147 (82). A few tokens are two memory accesses, a barrier and one more; prompts are bound by
+// how few pages they are (500, 16 waves each), and past 16000 tokens by the map: each page, or
+// each two that begin in one block, reads all of it, in every block of its heads.
 // Before the one-row form, with a page's heads to a wave each, 1536 tokens took 15.4; with
 // conversions through fp32 and the map read token by token, prompts of 8 x 1000 took 43.
 struct ScaledWrite {
