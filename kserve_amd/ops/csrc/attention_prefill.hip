@@ -176,8 +176,8 @@ extern "C" int ks_context_scaled_splits(int num_seqs, long rows, int max_q_len, 
                                         int Hkv, int max_nb, int window) {
   if (num_seqs < 1 || max_q_len < 1 || Hkv < 1 || Hq % Hkv != 0) return 1;
   if (ks_scaled_few_columns(max_q_len, Hq / Hkv) > 0) {
-    if (window > 0 && max_nb > (window + max_q_len) / PAGE + 2)
-      max_nb = (window + max_q_len) / PAGE + 2;
+    const long seen = ((long)window + max_q_len) / PAGE + 2;
+    if (window > 0 && max_nb > seen) max_nb = (int)seen;
     return ks_scaled_few_splits(num_seqs, max_q_len, Hq, Hkv, max_nb);
   }
   return ks_context_prefill_splits(num_seqs, rows, max_q_len, Hq, Hkv, max_nb, window);

@@ -446,3 +446,14 @@ def test_decode_behind_a_window(native, seqs, window):
     assert splits <= max(-(-pairs // 4), pairs // 128, 1)
     if seqs < 24 and pairs <= (32 if seqs >= 12 else 16):
         assert (waves, splits) == (8, 1)
+
+
+@pytest.mark.parametrize("window", [0, 2000, (1 << 31) - 20])
+def test_few_queries_behind_a_window(native, window):
+    """Block-scaled attention of few queries: as many key parts as what they see has, of
+    windows near the largest integer too."""
+    rule = native.ks_context_scaled_splits
+    rule.argtypes = [ctypes.c_int, ctypes.c_long] + [ctypes.c_int] * 5
+    wide = (1 << 27) - 1  # pages of a table
+    want = rule(1, 5 * 8, 5, 8, 8, min(wide, window // 16 + 2 if window else wide), 0)
+    assert rule(1, 5 * 8, 5, 8, 8, wide, window) == want > 1
