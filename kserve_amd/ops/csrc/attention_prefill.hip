@@ -39,7 +39,7 @@
 // Block-scaled E4M3 pages: a wave's 16 rows of a tile are one page, so its power of two is one
 // operand of the conversions that widen them between registers and LDS, and is applied
 // exactly. That widening is what they cost (2 x 1000 queries over 13000 keys, us: 430 to 510 by
-// box, bf16 pages 400 beside 510; without the conversions 435, without the LDS writes 460,
+// card, bf16 pages 400 beside 510; without the conversions 435, without the LDS writes 460,
 // without both 410); K as bytes into the products that take E8M0 scales themselves was 5%
 // faster, but sums products in less than 32 bits. Few queries go to attention_scaled.hip.
 //

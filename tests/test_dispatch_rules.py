@@ -448,7 +448,7 @@ def test_decode_behind_a_window(native, seqs, window):
         assert (waves, splits) == (8, 1)
 
 
-@pytest.mark.parametrize("window", [0, 2000, (1 << 31) - 20])
+@pytest.mark.parametrize("window", [0, 2000, (1 << 31) - 20, (1 << 31) - 3])
 def test_few_queries_behind_a_window(native, window):
     """Block-scaled attention of few queries: as many key parts as what they see has, of
     windows near the largest integer too."""
