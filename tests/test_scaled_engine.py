@@ -506,3 +506,24 @@ class TestSplitHeads:
         else:
             with pytest.raises(ValueError):
                 r.allocate_kv_cache(16)
+
+
+class TestSpeculation:
+    @pytest.mark.parametrize("dev", devices())
+    def test_generates(self, dev, monkeypatch):
+        """Drafts found in the prompts, verified over the cache; refused rows are written over."""
+        e = engine("fp8_scaled", dev, block_size=16)
+        e.config.scheduler.speculative_ngram = 3
+        calls = []
+        verify = e.runner.execute_verify
+
+        def counted(batch, drafts, manager):
+            calls.append(sum(map(len, drafts)))
+            return verify(batch, drafts, manager)
+
+        monkeypatch.setattr(e.runner, "execute_verify", counted)
+        Watch(e.runner, monkeypatch)
+        prompts = [[5, 6, 7, 8] * 12, [3, 4] * 20]
+        out = e.generate(prompts, SamplingParams(temperature=0.0, max_tokens=20))
+        assert all(len(o.output_token_ids) == 20 for o in out.values())
+        assert sum(calls) > 0
